@@ -40,7 +40,8 @@ typedef enum mlb_dtype {
     MLB_DT_DEFAULT = 0,      /* as the file's config says (float32 when it says nothing) */
     MLB_DT_F32 = 1,
     MLB_DT_BF16 = 2,
-    MLB_DT_FP8_E4M3 = 3      /* weights only: per-output-row fp32 scale = max|row|/448 */
+    MLB_DT_FP8_E4M3 = 3,     /* weights only: per-output-row fp32 scale = max|row|/448 */
+    MLB_DT_FP4_E2M1 = 4      /* pages of mlb_paged_kv only: an e4m3 scale per 16 values  */
 } mlb_dtype;
 
 typedef enum mlb_layer_type { MLB_LAYER_ATTENTION = 0, MLB_LAYER_DELTA_NET = 1 } mlb_layer_type;
@@ -277,6 +278,73 @@ size_t mlb_op_attn_decode_static_capacity(void);
  * error code the way those kernels do. Returns MLB_E_TIMEOUT (the expected outcome) once the
  * kernel has ended; the CUDA context stays usable. */
 int mlb_op_wait_probe(int device, uint32_t max_polls);
+
+/* ---- operators over a caller's paged K/V cache -----------------------------------------------------------------
+ * No counterpart in the reference, which keeps no cache. They are for programs that own their pages and run their own
+ * model around them: fill pages with the rows of new tokens, attend to pages, read rows back. All pointers inside are DEVICE
+ * memory of the handle's device; the calls run on `stream` (a cudaStream_t of that device, NULL = its default stream),
+ * whatever device is current, do not wait for it, allocate nothing and can be captured into a CUDA graph.
+ *
+ * mlb_ops holds what the kernels need beside the caller's buffers: an error word and 20 MB of scratch for partial
+ * results. Calls on one handle (graphs that captured them included) share both, so they must not overlap on the GPU: a
+ * handle per stream. Handles and graphs that captured calls on them are freed by the caller, the graphs first.
+ * mlb_ops_status waits for `stream` and reports what the kernels met since the last mlb_ops_status (MLB_E_INVALID: a page
+ * id outside the pools, a sequence longer than its row of the page table, a row_start that is no increasing sequence in
+ * 0..rows, more rows than max_rows, a position outside the rotation table); what such a sequence should have
+ * written is left as it was or, for a bad page id, computed from page 0 (a read) or left out (a write). */
+typedef struct mlb_ops mlb_ops;
+int mlb_ops_new(int device, mlb_ops** out);
+void mlb_ops_free(mlb_ops* o);
+int mlb_ops_status(mlb_ops* o, void* stream);
+
+/* A paged cache, the layout of mlb_op_attn_decode. Pools start on 16 bytes.
+ *   float32, bfloat16: [num_pages][kv_heads][16][head_dim]
+ *   fp4_e2m1: codes [num_pages][kv_heads][16][head_dim / 2] bytes (the even dim in the low half) and e4m3 scales
+ *   [num_pages][kv_heads][16][head_dim / 16]; a value is code * scale * k_scale (or v_scale: one positive factor per
+ *   pool, so that the scales of its blocks lie well inside e4m3's range; 1 where nothing is known).
+ * head_dim 64 or 128. page_table [batch][pt_stride]; entries behind a sequence's last page are not read. */
+typedef struct mlb_paged_kv {
+    void *kpool, *vpool;
+    void *kscale, *vscale;   /* fp4_e2m1 only, else ignored                                 */
+    const int32_t* page_table;
+    int32_t pt_stride, num_pages, kv_heads, head_dim;
+    int32_t dtype;           /* mlb_dtype                                                  */
+    float k_scale, v_scale;  /* fp4_e2m1 only, else ignored                                 */
+} mlb_paged_kv;
+
+/* The new tokens of a call. Sequence b brings rows row_start[b] .. row_start[b + 1] - 1 of the call's row tensors (row_start
+ * NULL: row b alone), the last of which stands at position kv_lens[b] - 1: kv_lens counts cached positions with the
+ * new ones. A row whose position would be negative (kv_lens[b] smaller than the number of rows) is padding: it attends to nothing
+ * (its output is 0) and is neither stored nor rotated. Rows that belong to no sequence are left as they were. */
+typedef struct mlb_new_rows {
+    const int32_t* row_start; /* [batch + 1] or NULL                                         */
+    const int32_t* kv_lens;   /* [batch]                                                     */
+    int32_t batch;            /* 1 .. 4096                                                   */
+    int32_t rows;             /* rows of the row tensors                                     */
+    int32_t max_rows;         /* no sequence brings more than these; 0 = not known           */
+} mlb_new_rows;
+
+/* Writes k and v [rows][kv_heads * head_dim] (row_dtype float32 or bfloat16; strides in elements from row to row) to
+ * the pages of their positions. With a table rope [rope_len][head_dim] of interleaved (cos, sin) as mlb_rope_table makes
+ * it, dims 2i and 2i + 1 of k are turned by the table row of the position first; so is q [rows][heads * head_dim], where
+ * given, into q_out (which may be q). Each product and sum of the rotation is one fp32 operation. In a 4-bit cache 16 dims
+ * get the scale e4m3(max|x| / (6 k_scale)) and the codes nearest to x * (1 / (scale * k_scale)), ties to the even code; an
+ * infinity takes the largest code and scale, a NaN is stored as some number. Two sequences must not append to one page. */
+int mlb_op_kv_append(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows, int row_dtype, const void* k,
+                     int64_t k_stride, const void* v, int64_t v_stride, const float* rope_or_null, int rope_len,
+                     const void* q_or_null, int64_t q_stride, void* q_out, int64_t q_out_stride, int heads, void* stream);
+/* The reverse: the rows' cached keys and values (as rotated and rounded) to k_out and v_out [rows][kv_heads * head_dim]. */
+int mlb_op_kv_read(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows, int row_dtype, void* k_out,
+                   int64_t k_stride, void* v_out, int64_t v_stride, void* stream);
+/* Causal attention of the rows (already in the cache) over the pages: the row at position p sees position j <= p where
+ * window = 0, or j > p - window (its newest `window` positions, itself among them), or j < sinks (the first ones). q and out
+ * [rows][heads * head_dim] of row_dtype, heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
+ * (0: 1 / sqrt(head_dim)); gate (nullable) fp32 [rows][heads * head_dim] multiplies the output. Sums and softmax statistics are
+ * fp32; with float32 rows so is everything else to fp32's own rounding, with bfloat16 rows probabilities may be rounded to bf16. What
+ * lies at positions that a row does not see (numbers or not) does not reach its output. */
+int mlb_op_attn_paged(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows, int row_dtype, const void* q,
+                      int64_t q_stride, const float* gate_or_null, void* out, int64_t out_stride, int heads, float scale,
+                      int window, int sinks, void* stream);
 
 /* RoPE table exactly as getPreComputedRopeTheta builds it (inference.h:4,
  * inference.cu:364-374): [max_len][head_dim] interleaved (cos, sin), host float math. */

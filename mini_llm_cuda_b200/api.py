@@ -16,7 +16,7 @@ MLB_MAX_LAYERS = 128
 MLB_OK = 0
 MLB_E_INVALID, MLB_E_IO, MLB_E_FORMAT, MLB_E_CUDA, MLB_E_NOMEM = -1, -2, -3, -4, -5
 MLB_E_KV_FULL, MLB_E_CONTEXT_FULL, MLB_E_TIMEOUT, MLB_E_UNSUPPORTED = -6, -7, -8, -9
-DT_DEFAULT, DT_F32, DT_BF16, DT_FP8 = 0, 1, 2, 3
+DT_DEFAULT, DT_F32, DT_BF16, DT_FP8, DT_FP4 = 0, 1, 2, 3, 4
 _DTYPE_NAMES = {"float32": DT_F32, "bfloat16": DT_BF16, "float8_e4m3": DT_FP8}
 
 
@@ -42,6 +42,17 @@ class Config(C.Structure):
 class Sampling(C.Structure):
     _fields_ = [("mode", C.c_int32), ("top_k", C.c_int32), ("temperature", C.c_float),
                 ("seeds", C.POINTER(C.c_uint64))]
+
+
+class PagedKvStruct(C.Structure):
+    _fields_ = [("kpool", C.c_void_p), ("vpool", C.c_void_p), ("kscale", C.c_void_p), ("vscale", C.c_void_p),
+                ("page_table", C.c_void_p), ("pt_stride", C.c_int32), ("num_pages", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("k_scale", C.c_float), ("v_scale", C.c_float)]
+
+
+class NewRowsStruct(C.Structure):
+    _fields_ = [("row_start", C.c_void_p), ("kv_lens", C.c_void_p), ("batch", C.c_int32), ("rows", C.c_int32),
+                ("max_rows", C.c_int32)]
 
 
 class KernelStat(C.Structure):
@@ -112,6 +123,13 @@ def lib() -> C.CDLL:
                                                 C.c_int, C.c_int, C.c_int, vp]),
         "mlb_op_attn_decode_static_status": (C.c_int, [vp]),
         "mlb_op_attn_decode_static_capacity": (C.c_size_t, []),
+        "mlb_ops_new": (C.c_int, [C.c_int, C.POINTER(vp)]),
+        "mlb_ops_free": (None, [vp]),
+        "mlb_ops_status": (C.c_int, [vp, vp]),
+        "mlb_op_kv_append": (C.c_int, [vp, vp, vp, C.c_int, vp, C.c_int64, vp, C.c_int64, vp, C.c_int, vp, C.c_int64, vp, C.c_int64,
+                                       C.c_int, vp]),
+        "mlb_op_kv_read": (C.c_int, [vp, vp, vp, C.c_int, vp, C.c_int64, vp, C.c_int64, vp]),
+        "mlb_op_attn_paged": (C.c_int, [vp, vp, vp, C.c_int, vp, C.c_int64, vp, vp, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_int, vp]),
         "mlb_last_error": (C.c_char_p, []),
         "mlb_version": (C.c_char_p, []),
         "mlb_compat_configure": (C.c_int, [cfgp, C.c_int]),
@@ -385,6 +403,151 @@ class Pool:
     def close(self):
         if self._h:
             lib().mlb_pool_free(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+_ROW_DTYPES = {"torch.float32": DT_F32, "torch.bfloat16": DT_BF16}
+_CACHE_DTYPES = {**_ROW_DTYPES, "torch.uint8": DT_FP4}
+
+
+def _dense(x, what: str, dtypes, shape=None):
+    if str(x.dtype) not in dtypes:
+        raise ValueError(f"{what} is {x.dtype}: expected one of {', '.join(dtypes)}")
+    if not x.is_cuda or not x.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous tensor on a CUDA device")
+    if shape is not None and tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(x.shape)}: expected {tuple(shape)}")
+    return x
+
+
+class PagedKV:
+    """A paged K/V cache in CUDA tensors of the caller's (mlb_paged_kv): pools [num_pages][kv_heads][16][head_dim] in
+    fp32 or bf16, or [num_pages][kv_heads][16][head_dim / 2] bytes of two 4-bit codes with e4m3 scales
+    [num_pages][kv_heads][16][head_dim / 16]; page_table [batch][pages] int32. Keeps the tensors alive."""
+
+    def __init__(self, kpool, vpool, page_table, kscale=None, vscale=None, k_scale: float = 1.0, v_scale: float = 1.0):
+        _dense(kpool, "kpool", _CACHE_DTYPES)
+        _dense(vpool, "vpool", (str(kpool.dtype),), kpool.shape)
+        _dense(page_table, "page_table", ("torch.int32",))
+        if kpool.dim() != 4 or kpool.shape[2] != 16 or page_table.dim() != 2:
+            raise ValueError("pools are [num_pages][kv_heads][16][...], a page table [batch][pages]")
+        self.dtype = _CACHE_DTYPES[str(kpool.dtype)]
+        pages, self.kv_heads, _, width = kpool.shape
+        self.head_dim = width * 2 if self.dtype == DT_FP4 else width
+        if self.dtype == DT_FP4:
+            if kscale is None or vscale is None:
+                raise ValueError("a 4-bit cache has scales")
+            for x, what in ((kscale, "kscale"), (vscale, "vscale")):
+                _dense(x, what, ("torch.float8_e4m3fn", "torch.uint8"), (pages, self.kv_heads, 16, self.head_dim // 16))
+        self.batch = page_table.shape[0]
+        self.tensors = [t for t in (kpool, vpool, page_table, kscale, vscale) if t is not None]
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        self.struct = PagedKvStruct(ptr(kpool), ptr(vpool), ptr(kscale), ptr(vscale), ptr(page_table), page_table.shape[1], pages,
+                                    self.kv_heads, self.head_dim, self.dtype, k_scale, v_scale)
+        self.ref = C.byref(self.struct)
+
+
+class NewRows:
+    """The new tokens of a call (mlb_new_rows): sequence b brings rows row_start[b] .. row_start[b + 1] - 1 (without row_start:
+    row b), the last of them at position kv_lens[b] - 1. `max_rows`: most rows of a sequence, 0 where not known."""
+
+    def __init__(self, kv_lens, rows: int, row_start=None, max_rows: int = 0):
+        _dense(kv_lens, "kv_lens", ("torch.int32",))
+        self.batch, self.rows = kv_lens.numel(), int(rows)
+        if row_start is not None:
+            _dense(row_start, "row_start", ("torch.int32",), (self.batch + 1,))
+        self.tensors = [t for t in (kv_lens, row_start) if t is not None]
+        self.struct = NewRowsStruct(row_start.data_ptr() if row_start is not None else None, kv_lens.data_ptr(), self.batch, self.rows, max_rows)
+        self.ref = C.byref(self.struct)
+
+
+class Ops:
+    """Operators over paged caches on one device and stream (mlb_ops). Row tensors are [rows][heads * head_dim] (or
+    [rows][heads][head_dim]) fp32 or bf16 with any stride between rows; `stream` is a CUDA stream's handle (0: the default
+    stream). Calls do not wait for the stream; status() does, and raises for what the kernels found wrong with the data."""
+
+    def __init__(self, device: int = 0):
+        self._h = C.c_void_p()
+        self.device = device
+        check(lib().mlb_ops_new(device, C.byref(self._h)))
+        L = lib()
+        self._append, self._read, self._attn = L.mlb_op_kv_append, L.mlb_op_kv_read, L.mlb_op_attn_paged
+
+    def _rows(self, x, what: str, rows: NewRows, width: int, dtype=None):
+        """(pointer, stride) of a row tensor."""
+        if dtype is not None and x.dtype != dtype:
+            raise ValueError(f"{what} is {x.dtype}: expected {dtype}")
+        shape = x.shape
+        if x.get_device() != self.device:
+            raise ValueError(f"{what} is not on CUDA device {self.device}")
+        inner = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else -1
+        if shape[0] != rows.rows or inner != width or x.stride(-1) != 1 or (len(shape) == 3 and x.stride(1) != shape[2]):
+            raise ValueError(f"{what} must be [{rows.rows}][{width}], dense within a row")
+        return x.data_ptr(), x.stride(0)
+
+    def _check(self, cache: PagedKV, rows: NewRows, x, what: str) -> int:
+        if cache.batch < rows.batch:
+            raise ValueError(f"the page table has {cache.batch} rows, the call {rows.batch} sequences")
+        for t in cache.tensors + rows.tensors:
+            if t.get_device() != self.device:
+                raise ValueError(f"the cache and its rows must be on CUDA device {self.device}")
+        dt = _ROW_DTYPES.get(str(x.dtype))
+        if dt is None:
+            raise ValueError(f"{what} is {x.dtype}: expected float32 or bfloat16")
+        return dt
+
+    def kv_append(self, cache: PagedKV, rows: NewRows, k, v, rope=None, q=None, q_out=None, heads: int = 0, stream: int = 0):
+        """Rotates k (and q into q_out, which may be q) by the rows' positions and writes k and v to their pages."""
+        dt = self._check(cache, rows, k, "k")
+        width = cache.kv_heads * cache.head_dim
+        kp, ks = self._rows(k, "k", rows, width)
+        vp_, vs = self._rows(v, "v", rows, width, k.dtype)
+        qp, qs, op, os_ = None, 0, None, 0
+        if q is not None:
+            qp, qs = self._rows(q, "q", rows, heads * cache.head_dim, k.dtype)
+            op, os_ = self._rows(q_out, "q_out", rows, heads * cache.head_dim, k.dtype)
+        rp, rl = None, 0
+        if rope is not None:
+            _dense(rope, "rope", ("torch.float32",), (rope.shape[0], cache.head_dim))
+            if rope.get_device() != self.device:
+                raise ValueError(f"rope is not on CUDA device {self.device}")
+            rp, rl = rope.data_ptr(), rope.shape[0]
+        check(self._append(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, rp, rl, qp, qs, op, os_, heads, stream))
+
+    def kv_read(self, cache: PagedKV, rows: NewRows, k_out, v_out, stream: int = 0):
+        """The rows' cached keys and values, as values."""
+        dt = self._check(cache, rows, k_out, "k_out")
+        width = cache.kv_heads * cache.head_dim
+        kp, ks = self._rows(k_out, "k_out", rows, width)
+        vp_, vs = self._rows(v_out, "v_out", rows, width, k_out.dtype)
+        check(self._read(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, stream))
+
+    def attn_paged(self, cache: PagedKV, rows: NewRows, q, out, heads: int, gate=None, scale: float = 0.0, window: int = 0, sinks: int = 0,
+                   stream: int = 0):
+        """Causal attention of the rows, optionally within a window and to the first `sinks` positions (mlb_op_attn_paged)."""
+        dt = self._check(cache, rows, q, "q")
+        width = heads * cache.head_dim
+        qp, qs = self._rows(q, "q", rows, width)
+        op, os_ = self._rows(out, "out", rows, width, q.dtype)
+        gp = None
+        if gate is not None:
+            _dense(gate, "gate", ("torch.float32",))
+            gp, gs = self._rows(gate, "gate", rows, width)
+        check(self._attn(self._h, cache.ref, rows.ref, dt, qp, qs, gp, op, os_, heads, scale, window, sinks, stream))
+
+    def status(self, stream: int = 0):
+        """Waits for the stream; raises if a call since the last status() met a bad page id, row range or length."""
+        check(lib().mlb_ops_status(self._h, stream))
+
+    def close(self):
+        if self._h:
+            lib().mlb_ops_free(self._h)
             self._h = C.c_void_p()
 
     def __del__(self):

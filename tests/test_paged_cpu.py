@@ -1,0 +1,120 @@
+"""Refusals of the operators over a caller's paged K/V cache: arguments are checked before the handle, so no GPU is needed."""
+import ctypes as C
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def api(built_lib):
+    from mini_llm_cuda_b200 import api as _api
+    return _api
+
+
+def cache(api, **kw):
+    d = dict(kpool=4096, vpool=8192, kscale=None, vscale=None, page_table=64, pt_stride=4, num_pages=9, kv_heads=2, head_dim=64,
+             dtype=api.DT_BF16, k_scale=1.0, v_scale=1.0)
+    d.update(kw)
+    return api.PagedKvStruct(**d)
+
+
+def new_rows(api, **kw):
+    d = dict(row_start=None, kv_lens=128, batch=3, rows=3, max_rows=0)
+    d.update(kw)
+    return api.NewRowsStruct(**d)
+
+
+def calls(api, kv, rows, dt=None, ptr=1 << 20, stride=1 << 10):
+    """Status of each operator with these descriptions and no handle."""
+    L, dt = api.lib(), api.DT_BF16 if dt is None else dt
+    kvp, rp = C.byref(kv) if kv is not None else None, C.byref(rows) if rows is not None else None
+    return [L.mlb_op_kv_append(None, kvp, rp, dt, ptr, stride, ptr, stride, None, 0, None, 0, None, 0, 0, None),
+            L.mlb_op_kv_read(None, kvp, rp, dt, ptr, stride, ptr, stride, None),
+            L.mlb_op_attn_paged(None, kvp, rp, dt, ptr, stride, None, ptr, stride, 4, 0.0, 0, 0, None)]
+
+
+def test_without_a_handle(api):
+    assert calls(api, cache(api), new_rows(api)) == [api.MLB_E_INVALID] * 3
+    assert b"null handle" in api.lib().mlb_last_error()
+    assert calls(api, None, new_rows(api)) == [api.MLB_E_INVALID] * 3
+    assert calls(api, cache(api), None) == [api.MLB_E_INVALID] * 3
+    assert api.lib().mlb_ops_status(None, None) == api.MLB_E_INVALID
+    assert api.lib().mlb_ops_new(0, None) == api.MLB_E_INVALID
+    api.lib().mlb_ops_free(None)
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(kpool=None), "INVALID", b"null pointer"),
+    (dict(page_table=None), "INVALID", b"null pointer"),
+    (dict(dtype=3), "INVALID", b"float32, bfloat16 or fp4"),
+    (dict(dtype=0), "INVALID", b"float32, bfloat16 or fp4"),
+    (dict(dtype=4), "INVALID", b"has scales"),
+    (dict(dtype=4, kscale=256, vscale=512, k_scale=0.0), "INVALID", b"positive"),
+    (dict(dtype=4, kscale=256, vscale=512, v_scale=float("nan")), "INVALID", b"positive"),
+    (dict(dtype=4, kscale=256, vscale=512, v_scale=float("inf")), "INVALID", b"positive"),
+    (dict(dtype=4, kscale=257, vscale=512), "INVALID", b"16 bytes"),
+    (dict(kpool=4104), "INVALID", b"16 bytes"),
+    (dict(pt_stride=0), "INVALID", b">= 1"),
+    (dict(pt_stride=1 << 27), "UNSUPPORTED", b"pt_stride"),
+    (dict(num_pages=0), "INVALID", b">= 1"),
+    (dict(kv_heads=0), "INVALID", b">= 1"),
+    (dict(head_dim=96), "UNSUPPORTED", b"64 or 128"),
+])
+def test_refused_caches(api, kw, status, text):
+    want = getattr(api, "MLB_E_" + status)
+    assert calls(api, cache(api, **kw), new_rows(api)) == [want] * 3
+    assert text in api.lib().mlb_last_error()
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(kv_lens=None), "INVALID"), (dict(batch=0), "INVALID"), (dict(batch=4097), "INVALID"), (dict(rows=-1), "INVALID"),
+    (dict(max_rows=-1), "INVALID"), (dict(rows=1 << 30), "UNSUPPORTED"),
+])
+def test_refused_rows(api, kw, status):
+    assert calls(api, cache(api), new_rows(api, **kw)) == [getattr(api, "MLB_E_" + status)] * 3
+
+
+def test_refused_row_tensors(api):
+    kv, rows = cache(api), new_rows(api)
+    assert calls(api, kv, rows, dt=api.DT_FP8) == [api.MLB_E_INVALID] * 3
+    assert calls(api, kv, rows, ptr=None) == [api.MLB_E_INVALID] * 3
+    assert calls(api, kv, rows, ptr=(1 << 20) + 1) == [api.MLB_E_INVALID] * 3
+    assert calls(api, kv, rows, stride=127) == [api.MLB_E_INVALID] * 3
+    assert b"stride" in api.lib().mlb_last_error()
+    # no rows: nothing is looked at but the handle
+    assert calls(api, kv, new_rows(api, rows=0), ptr=None) == [api.MLB_E_INVALID] * 3
+    assert b"null handle" in api.lib().mlb_last_error()
+
+
+def test_refused_attention(api):
+    L, kv, rows, p = api.lib(), cache(api), new_rows(api), 1 << 20
+
+    def status(heads=4, scale=0.0, window=0, sinks=0, gate=None):
+        return L.mlb_op_attn_paged(None, C.byref(kv), C.byref(rows), api.DT_BF16, p, 4096, gate, p, 4096, heads, scale, window, sinks, None)
+
+    assert status(heads=3) == api.MLB_E_INVALID
+    assert status(heads=0) == api.MLB_E_INVALID
+    assert status(heads=18) == api.MLB_E_UNSUPPORTED
+    for kw in (dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(gate=2)):
+        assert status(**kw) == api.MLB_E_INVALID
+        assert b"null handle" not in L.mlb_last_error()
+
+
+def test_refused_append(api):
+    L, kv, rows, p = api.lib(), cache(api), new_rows(api), 1 << 20
+
+    def status(rope=None, rope_len=0, q=None, q_out=None, heads=0):
+        return L.mlb_op_kv_append(None, C.byref(kv), C.byref(rows), api.DT_BF16, p, 4096, p, 4096, rope, rope_len, q, 4096, q_out, 4096, heads, None)
+
+    for kw in (dict(rope=4096, rope_len=0), dict(rope=4097, rope_len=5), dict(q=p, q_out=None, heads=4), dict(q=p, q_out=p, heads=0),
+               dict(q=p, q_out=p + 1, heads=4)):
+        assert status(**kw) == api.MLB_E_INVALID
+        assert b"null handle" not in L.mlb_last_error()
+
+
+def test_no_device(api):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("this machine has a GPU")
+    h = C.c_void_p()
+    assert api.lib().mlb_ops_new(0, C.byref(h)) == api.MLB_E_CUDA
+    assert not h.value
