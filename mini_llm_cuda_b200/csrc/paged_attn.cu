@@ -77,39 +77,838 @@ __device__ __noinline__ void careful_row(const AttnPagedParams& p, int b, int po
     }
 }
 
-template <typename KVT, typename RT, int HD>
-__global__ void __launch_bounds__(256) attn_paged_rows_kernel(const __grid_constant__ AttnPagedParams p) {
-    const int warp = (blockIdx.x * 256 + threadIdx.x) >> 5, row = warp / p.heads, h = warp % p.heads;
-    if (row >= p.r.rows) return;
-    int b = row;
-    if (p.r.row_start) {
-        b = 0;
-        while (b + 1 < p.r.batch && p.r.row_start[b + 1] <= row) ++b;
-    } else if (b >= p.r.batch) {
-        return;
+// ---- blocks of up to eight rows on matrix cores -------------------------------------------------------------------------
+// A warp takes pages of 16 positions of one K/V head for a block of up to 8 rows (new tokens x the query heads of the K/V head):
+//   S[16 positions][8 rows] = K Q^T      A = K, B = Q^T,  m16n8k16
+//   O^T[dims][8 rows] += V^T P^T         A = V^T, B = P^T
+// Nothing is staged in shared memory but Q: dims of a dot product and positions of a sum may come in any order, so a lane loads 16
+// bytes of a K row and uses them as its elements of two (fp32: one, 4 bits: eight) k-steps, and 16 bytes each of four V rows whose
+// 16-bit halves it pairs up with byte permutes. S lies with positions along the lanes and rows within them, as O does: a running maximum
+// and its rescaling need no exchange between lanes but the maximum itself, and that only when a score passes the old one by 2^8; P is
+// turned round by movmatrix.
+// fp32 numbers are taken in pieces whose products are exact: an fp32 query in three bf16 (4-bit pages: two halves, the row scaled by
+// a power of two to lie within their range), fp32 K and V in three bf16, a probability in as many as the rows' type needs. Products of
+// pieces below 2^-24 of the whole are left out. 4-bit codes times their e4m3 scale are exact halves.
+constexpr int kSplitWarps = 8;
+constexpr float kLazy = 8.f;         // log2 of how far a score may pass the running maximum before it is moved
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t y;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+// N bf16 (or half) pairs whose sum is the pair (x, y) to 8 N (11 N) bits
+template <bool F16, int N>
+__device__ __forceinline__ void pieces(float x, float y, uint32_t (&o)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        o[i] = F16 ? f32x2_to_f16(x, y) : f32x2_to_bf16(x, y);
+        if (i + 1 < N) {
+            x -= F16 ? f16_lo(o[i]) : __uint_as_float(o[i] << 16);
+            y -= F16 ? f16_hi(o[i]) : __uint_as_float(o[i] & 0xffff0000u);
+        }
     }
-    const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, true);
-    if (row < s.r0 || row >= s.r0 + s.n) return;
-    careful_row<KVT, RT, HD>(p, b, s.len - s.n + row - s.r0, row, h);
+}
+
+// What a lane (g = lane / 4, j = lane % 4) holds of a page's K and V rows. A k-step's slots 0, 1 are k = 2j, 2j + 1, slots 2, 3 k = 2j + 8, 2j + 9;
+// dim() says which dim stands there. V: block vb of the lane's dims and M-tile mt within it hold dims vdim() and the next one.
+template <typename KVT, int HD> struct PageFrag;
+
+template <int HD>
+struct PageFrag<bf16_t, HD> {
+    static constexpr int KP = 1;                             // pieces of K and V
+    static constexpr bool F16 = false;
+    uint4 k[2][HD / 32], v[HD / 64][4];
+    __device__ static int dim(int ks, int j, int slot) { return ks / 2 * 32 + j * 8 + ks % 2 * 4 + slot; }
+    __device__ static int vdim(int mt, int g) { return mt / 4 * 64 + g * 8 + mt % 4 * 2; }
+    __device__ __forceinline__ void load_k(const PagedCache& c, size_t base, int g, int j) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const bf16_t*>(c.kpool) + base * HD);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int b = 0; b < HD / 32; ++b) k[t][b] = __ldg(p + (t * 8 + g) * (HD / 8) + b * 4 + j);
+    }
+    __device__ __forceinline__ void load_v(const PagedCache& c, size_t base, int g, int j) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const bf16_t*>(c.vpool) + base * HD);
+#pragma unroll
+        for (int b = 0; b < HD / 64; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[b][i] = __ldg(p + (2 * j + (i & 1) + (i & 2) * 4) * (HD / 8) + b * 8 + g);
+    }
+    __device__ __forceinline__ void hide_v(int i) {          // row i of the lane's four holds no number that may be used
+#pragma unroll
+        for (int b = 0; b < HD / 64; ++b) v[b][i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void k_operand(int ks, uint32_t (&a)[1][4]) const {
+        const uint4 x = k[0][ks / 2], y = k[1][ks / 2];
+        a[0][0] = ks % 2 ? x.z : x.x; a[0][1] = ks % 2 ? y.z : y.x; a[0][2] = ks % 2 ? x.w : x.y; a[0][3] = ks % 2 ? y.w : y.y;
+    }
+    __device__ __forceinline__ void v_operand(int mt, uint32_t (&a)[1][4]) const {
+        auto word = [&](int i) {
+            const uint4& x = v[mt / 4][i];
+            return mt % 4 == 0 ? x.x : mt % 4 == 1 ? x.y : mt % 4 == 2 ? x.z : x.w;
+        };
+        a[0][0] = __byte_perm(word(0), word(1), 0x5410); a[0][1] = __byte_perm(word(0), word(1), 0x7632);
+        a[0][2] = __byte_perm(word(2), word(3), 0x5410); a[0][3] = __byte_perm(word(2), word(3), 0x7632);
+    }
+};
+
+template <int HD>
+struct PageFrag<float, HD> {
+    static constexpr int KP = 3;
+    static constexpr bool F16 = false;
+    float4 k[2][HD / 16], v[HD / 32][4];
+    __device__ static int dim(int ks, int j, int slot) { return ks * 16 + j * 4 + slot; }
+    __device__ static int vdim(int mt, int g) { return mt / 2 * 32 + g * 4 + mt % 2 * 2; }
+    __device__ __forceinline__ void load_k(const PagedCache& c, size_t base, int g, int j) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(c.kpool) + base * HD);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int b = 0; b < HD / 16; ++b) k[t][b] = __ldg(p + (t * 8 + g) * (HD / 4) + b * 4 + j);
+    }
+    __device__ __forceinline__ void load_v(const PagedCache& c, size_t base, int g, int j) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(c.vpool) + base * HD);
+#pragma unroll
+        for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[b][i] = __ldg(p + (2 * j + (i & 1) + (i & 2) * 4) * (HD / 4) + b * 8 + g);
+    }
+    __device__ __forceinline__ void hide_v(int i) {
+#pragma unroll
+        for (int b = 0; b < HD / 32; ++b) v[b][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __device__ __forceinline__ void k_operand(int ks, uint32_t (&a)[3][4]) const {
+        uint32_t w[4][3];
+        pieces<false, 3>(k[0][ks].x, k[0][ks].y, w[0]);
+        pieces<false, 3>(k[1][ks].x, k[1][ks].y, w[1]);
+        pieces<false, 3>(k[0][ks].z, k[0][ks].w, w[2]);
+        pieces<false, 3>(k[1][ks].z, k[1][ks].w, w[3]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[i][e] = w[e][i];
+    }
+    __device__ __forceinline__ void v_operand(int mt, uint32_t (&a)[3][4]) const {
+        uint32_t w[4][3];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {                        // a0, a1: keys 2j, 2j + 1 of the two dims; a2, a3: keys 2j + 8, 2j + 9
+            const float4 &x = v[mt / 2][h / 2 * 2], &y = v[mt / 2][h / 2 * 2 + 1];
+            const float u = mt % 2 ? (h % 2 ? x.w : x.z) : (h % 2 ? x.y : x.x), z = mt % 2 ? (h % 2 ? y.w : y.z) : (h % 2 ? y.y : y.x);
+            pieces<false, 3>(u, z, w[h]);
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[i][e] = w[e][i];
+    }
+};
+
+template <int HD>
+struct PageFrag<fp4_t, HD> {
+    static constexpr bool F16 = true;
+    static constexpr int KW = HD / 32, VW = HD / 64;         // words of codes of a K row per lane, of a V row
+    uint32_t k[2][KW], ks_[2], v[4][VW], vs[2];
+    __device__ static int dim(int ks, int j, int slot) { return j * (HD / 4) + ks * 4 + slot; }
+    __device__ static int vdim(int mt, int g) { return g * (HD / 8) + mt * 2; }
+    __device__ __forceinline__ void load_k(const PagedCache& c, size_t base, int g, int j) {
+        const unsigned char *p = static_cast<const unsigned char*>(c.kpool) + base * (HD / 2), *s = c.kscale + base * (HD / 16);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int row = t * 8 + g;
+            if constexpr (HD == 128) {
+                const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + row * 64) + j);
+                k[t][0] = x.x; k[t][1] = x.y; k[t][2 % KW] = x.z; k[t][3 % KW] = x.w;
+                ks_[t] = __ldg(reinterpret_cast<const unsigned short*>(s + row * 8) + j);
+            } else {
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(p + row * 32) + j);
+                k[t][0] = x.x; k[t][1] = x.y;
+                ks_[t] = __ldg(s + row * 4 + j);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const PagedCache& c, size_t base, int g, int j) {
+        const unsigned char *p = static_cast<const unsigned char*>(c.vpool) + base * (HD / 2), *s = c.vscale + base * (HD / 16);
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 2 * j + (i & 1) + (i & 2) * 4;
+            if constexpr (HD == 128) {
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(p + row * 64) + g);
+                v[i][0] = x.x; v[i][1 % VW] = x.y;
+                b[i] = __ldg(s + row * 8 + g);
+            } else {
+                v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(p + row * 32) + g);
+                b[i] = __ldg(s + row * 4 + g / 2);
+            }
+        }
+        vs[0] = b[0] | b[1] << 8;
+        vs[1] = b[2] | b[3] << 8;
+    }
+    __device__ __forceinline__ void hide_v(int i) {          // (codes are numbers, but a scale's byte may be a NaN)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) v[i][w] = 0;
+        vs[i / 2] &= i % 2 ? 0x00ffu : 0xff00u;
+    }
+    // all k-steps at once: h[t][i] = two dims of row t * 8 + g
+    __device__ __forceinline__ void widen_k(uint32_t (&h)[2][HD / 8]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t s = e4m3x2_to_f16(ks_[t]), s0 = __byte_perm(s, s, 0x1010), s1 = __byte_perm(s, s, 0x3232);
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                uint32_t o[4];
+                e2m1x8_to_f16(k[t][w], o);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[t][w * 4 + i] = hmul2(o[i], w < 2 ? s0 : s1);
+            }
+        }
+    }
+};
+
+// Scores of a page: s[0..1] position g of rows 2j, 2j + 1, s[2..3] position g + 8. `qf` holds the rows' pieces as B operands: [piece][k-step][lane].
+template <typename KVT, int HD, int QP>
+__device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const uint2* qf, int lane, float (&s)[4]) {
+    using F = PageFrag<KVT, HD>;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};                       // two chains of products
+    s[0] = s[1] = s[2] = s[3] = 0.f;
+    if constexpr (F::F16) {
+        uint32_t h[2][HD / 8];
+        f.widen_k(h);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+            for (int i = 0; i < QP; ++i) {
+                const uint2 b = qf[(i * (HD / 16) + ks) * 32 + lane];
+                mma_f16(ks % 2 ? t : s, h[0][2 * ks], h[1][2 * ks], h[0][2 * ks + 1], h[1][2 * ks + 1], b.x, b.y);
+            }
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+            uint32_t a[F::KP][4];
+            f.k_operand(ks, a);
+#pragma unroll
+            for (int i = 0; i < QP; ++i) {
+                const uint2 b = qf[(i * (HD / 16) + ks) * 32 + lane];
+#pragma unroll
+                for (int k = 0; k < F::KP; ++k)
+                    if (i + k < 3) mma_bf16((ks + i) % 2 ? t : s, a[k][0], a[k][1], a[k][2], a[k][3], b.x, b.y);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += t[e];
+}
+
+// acc[mt]: dims vdim(mt, g) of rows 2j, 2j + 1 in [0], [1], the next dim in [2], [3]
+template <typename KVT, int HD, int PP>
+__device__ __forceinline__ void page_values(const PageFrag<KVT, HD>& f, const float (&w)[4], float (&acc)[HD / 16][4]) {
+    using F = PageFrag<KVT, HD>;
+    uint32_t p0[PP], p1[PP];
+    pieces<F::F16, PP>(w[0], w[1], p0);
+    pieces<F::F16, PP>(w[2], w[3], p1);
+#pragma unroll
+    for (int i = 0; i < PP; ++i) {
+        p0[i] = movmatrix(p0[i]);
+        p1[i] = movmatrix(p1[i]);
+    }
+    if constexpr (F::F16) {
+        const uint32_t s0 = e4m3x2_to_f16(f.vs[0]), s1 = e4m3x2_to_f16(f.vs[1]);
+#pragma unroll
+        for (int w8 = 0; w8 < F::VW; ++w8) {
+            uint32_t h[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e2m1x8_to_f16(f.v[i][w8], h[i]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const uint32_t a0 = hmul2(__byte_perm(h[0][m], h[1][m], 0x5410), s0), a1 = hmul2(__byte_perm(h[0][m], h[1][m], 0x7632), s0);
+                const uint32_t a2 = hmul2(__byte_perm(h[2][m], h[3][m], 0x5410), s1), a3 = hmul2(__byte_perm(h[2][m], h[3][m], 0x7632), s1);
+#pragma unroll
+                for (int i = 0; i < PP; ++i) mma_f16(acc[w8 * 4 + m], a0, a1, a2, a3, p0[i], p1[i]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int mt = 0; mt < HD / 16; ++mt) {
+            uint32_t a[F::KP][4];
+            f.v_operand(mt, a);
+#pragma unroll
+            for (int k = 0; k < F::KP; ++k)
+#pragma unroll
+                for (int i = 0; i < PP; ++i)
+                    if (i + k < 3) mma_bf16(acc[mt], a[k][0], a[k][1], a[k][2], a[k][3], p0[i], p1[i]);
+        }
+    }
+}
+
+// A block of rows of one K/V head: rows first .. first + count - 1 of the sequence's (token, head) pairs, token by token
+struct Block {
+    int b, kvh, first, count;
+    PagedSeq s;
+};
+
+template <typename RT, bool F16, int QP, int HD, typename F>
+__device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Block& k, uint2* qf, float* qscale, int lane) {
+    const int g = lane >> 2, j = lane & 3;                   // the B operand's column is a row of the block
+    const bool in = g < k.count;
+    const int r = k.first + (in ? g : 0), row = k.s.r0 + r / p.group, h = k.kvh * p.group + r % p.group;
+    const RT* q = static_cast<const RT*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD;
+    float up = 1.f, down = 1.f;
+    if (F16) {
+        // a power of two that brings the row's largest magnitude to 256 .. 512, if it is a number
+        float top = 0.f;
+        for (int d = j; d < HD; d += 4) top = fmaxf(top, fabsf(Elem<RT>::get(q, d)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(-100, min(100, 8 - ((int)(__float_as_uint(top) >> 23) - 127)));
+        up = __uint_as_float((uint32_t)(127 + e) << 23);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+    if (j == 0) qscale[g] = p.scale * p.c.k_scale * 1.4426950408889634f * down;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = in ? Elem<RT>::get(q, F::dim(ks, j, e)) * up : 0.f;
+        uint32_t lo[QP], hi[QP];
+        pieces<F16, QP>(x[0], x[1], lo);
+        pieces<F16, QP>(x[2], x[3], hi);
+#pragma unroll
+        for (int i = 0; i < QP; ++i) qf[(i * (HD / 16) + ks) * 32 + lane] = make_uint2(lo[i], hi[i]);
+    }
+}
+
+template <typename KVT, typename RT, int HD>
+struct SplitShape {
+    using F = PageFrag<KVT, HD>;
+    static constexpr int QP = sizeof(RT) == 2 ? 1 : F::F16 ? 2 : 3;
+    static constexpr int PP = sizeof(RT) == 2 ? (F::F16 ? 1 : 2) : F::F16 ? 2 : 3;
+    static constexpr int QWORDS = QP * (HD / 16) * 32;       // uint2 of a warp's queries
+    static constexpr int W = HD + 2;                         // floats of a row's partial result: its sums, maximum, total
+    static constexpr int PART = 8 * W;
+};
+__host__ __device__ constexpr int split_part_floats(int hd) { return 8 * (hd + 2); }
+
+// The pages v, v + step, .. < v1 of a span for a block; results in acc, m (log2 of the reference of the weights) and l
+template <typename KVT, typename RT, int HD>
+__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, const uint2* qf,
+                                           const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
+    using S = SplitShape<KVT, RT, HD>;
+    const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+    if (v >= v1) return;
+    const int pos0 = k.s.len - k.s.n;
+    int pos[2];
+    pos[0] = 2 * j < k.count ? pos0 + (k.first + 2 * j) / p.group : -1;
+    pos[1] = 2 * j + 1 < k.count ? pos0 + (k.first + 2 * j + 1) / p.group : -1;
+    const int low = pos0 + k.first / p.group, high = pos0 + (k.first + k.count - 1) / p.group;      // positions of the block's rows
+    const float c0 = qscale[2 * j], c1 = qscale[2 * j + 1];
+    auto base_of = [&](int id) { return ((size_t)id * p.c.kv_heads + k.kvh) * kKvBlock; };
+    PageFrag<KVT, HD> f;
+    int id = paged_page(p.c, p.r.err, k.b, span.page(v), 0);
+    f.load_k(p.c, base_of(id), g, j);
+    int next = v + step < v1 ? paged_page(p.c, p.r.err, k.b, span.page(v + step), 0) : 0;
+#pragma unroll 1
+    for (; v < v1; v += step) {
+        const int key0 = span.page(v) * kKvBlock;
+        f.load_v(p.c, base_of(id), g, j);
+        float s[4];
+        page_scores<KVT, HD, S::QP>(f, qf, lane, s);
+        if (v + step < v1) f.load_k(p.c, base_of(next), g, j);
+        id = next;
+        if (v + 2 * step < v1) next = paged_page(p.c, p.r.err, k.b, span.page(v + 2 * step), 0);
+        s[0] *= c0; s[1] *= c1; s[2] *= c0; s[3] *= c1;
+        if (key0 + kKvBlock - 1 > low || (p.window > 0 && key0 <= high - p.window && key0 + kKvBlock > p.sinks)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!paged_sees(p, pos[e & 1], key0 + g + (e & 2) * 4)) s[e] = -INFINITY;
+            // 0 times what is no number is no number: values that no row sees become zeros
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = key0 + 2 * j + (i & 1) + (i & 2) * 4;
+                if (key > high || (p.window > 0 && key <= low - p.window && key >= p.sinks)) f.hide_v(i);
+            }
+        }
+        const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
+        if (__any_sync(0xffffffffu, t0 > m[0] + kLazy || t1 > m[1] + kLazy)) {
+            float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+            }
+            const float f0 = n0 == m[0] ? 1.f : ex2(m[0] - n0), f1 = n1 == m[1] ? 1.f : ex2(m[1] - n1);
+            m[0] = n0; m[1] = n1;
+            l[0] *= f0; l[1] *= f1;
+#pragma unroll
+            for (int t = 0; t < HD / 16; ++t) { acc[t][0] *= f0; acc[t][1] *= f1; acc[t][2] *= f0; acc[t][3] *= f1; }
+        }
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];      // (nothing seen yet)
+        s[0] = ex2(s[0] - r0); s[1] = ex2(s[1] - r1); s[2] = ex2(s[2] - r0); s[3] = ex2(s[3] - r1);
+        l[0] += s[0] + s[2];
+        l[1] += s[1] + s[3];
+        page_values<KVT, HD, S::PP>(f, s, acc);
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+        l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+    }
+}
+
+// Row i of a block: its row of the call's tensors, head, and position
+__device__ __forceinline__ void block_row(const AttnPagedParams& p, const Block& k, int i, int& row, int& h, int& pos) {
+    const int r = k.first + i, t = r / p.group;
+    row = k.s.r0 + t;
+    h = k.kvh * p.group + r % p.group;
+    pos = k.s.len - k.s.n + t;
+}
+
+// Result of dims d, d + 1 of a row: sums over the total. True if it is not finite (a row that sees nothing is 0).
+template <typename RT, int HD>
+__device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int h, int pos, int d, float x, float y, float l) {
+    const float inv = pos < 0 ? 0.f : p.c.v_scale / l;
+    x = pos < 0 ? 0.f : x * inv;
+    y = pos < 0 ? 0.f : y * inv;
+    const size_t at = (size_t)row * p.heads * HD + (size_t)h * HD + d;
+    const bool odd = !(fabsf(x) <= 3.4e38f) || !(fabsf(y) <= 3.4e38f);
+    if (p.gate) { x *= p.gate[at]; y *= p.gate[at + 1]; }
+    RT* o = static_cast<RT*>(p.out) + (size_t)row * p.out_stride + (size_t)h * HD + d;
+    if (reinterpret_cast<uintptr_t>(o) % (2 * sizeof(RT)) == 0) {
+        if constexpr (sizeof(RT) == 2) *reinterpret_cast<uint32_t*>(o) = f32x2_to_bf16(x, y);
+        else *reinterpret_cast<float2*>(o) = make_float2(x, y);
+    } else {
+        Elem<RT>::put(o, 0, x);
+        Elem<RT>::put(o, 1, y);
+    }
+    return odd;
+}
+
+// ---- the positions of all sequences dealt out evenly ---------------------------------------------------------------------
+// Page counts of a batch's sequences differ, and so does how many sequences there are for 148 SMs: so the pages of all (sequence, K/V
+// head, block of rows) are laid end to end and cut into as many equal shares as there are teams (a CTA's warps together, or each warp alone),
+// and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Sequences of more than
+// kSplitRows (token, head) pairs are left to the kernels for prompts.
+constexpr int kSplitRows = 32;
+
+// (sequences, pages of their items before them) -> plan in shared memory; returns the total
+__device__ __forceinline__ int split_blocks(const AttnPagedParams& p, int n) {
+    const long long rows = (long long)n * p.group;
+    return rows > kSplitRows ? 0 : (int)((rows + 7) / 8);
+}
+
+__device__ __forceinline__ unsigned long long share_start(unsigned long long total, int teams, int t) {
+    return total / (unsigned)teams * (unsigned)t + total % (unsigned)teams * (unsigned)t / (unsigned)teams;
+}
+__device__ __forceinline__ int split_teams(unsigned long long total, int max_teams, int min_pages) {
+    const unsigned long long n = total / (unsigned)min_pages;
+    return n < 1 ? 1 : n < (unsigned)max_teams ? (int)n : max_teams;
+}
+
+// TEAM: warps of a team, 1 or kSplitWarps
+template <typename KVT, typename RT, int HD, int TEAM>
+__global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const __grid_constant__ AttnPagedParams p) {
+    using S = SplitShape<KVT, RT, HD>;
+    extern __shared__ __align__(16) unsigned char sm[];
+    uint2* qf_all = reinterpret_cast<uint2*>(sm);                                        // [warp][QWORDS]
+    float* red = reinterpret_cast<float*>(sm + (size_t)kSplitWarps * S::QWORDS * 8);     // TEAM > 1: [warp][8][W], a row's maximum and total behind its sums
+    unsigned long long* plan = reinterpret_cast<unsigned long long*>(red + (TEAM > 1 ? kSplitWarps * S::PART : 0));      // [batch + 1]
+    __shared__ float qs_all[kSplitWarps][8];
+    __shared__ unsigned long long warp_sum_[kSplitWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
+    pdl_launch_dependents();
+    // pages before each sequence
+    unsigned long long before = 0;
+    for (int b0 = 0; b0 < p.r.batch; b0 += 32 * kSplitWarps) {
+        const int b = b0 + tid;
+        unsigned long long n = 0;
+        if (b < p.r.batch) {
+            const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0);
+            const int blocks = split_blocks(p, s.n);
+            if (blocks > 0) n = (unsigned long long)max(1, paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
+        }
+        unsigned long long x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_sum_[warp] = x;
+        __syncthreads();
+        unsigned long long all = 0, mine = 0;
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; ++w) {
+            if (w < warp) mine += warp_sum_[w];
+            all += warp_sum_[w];
+        }
+        if (b < p.r.batch) plan[b] = before + mine + x - n;
+        before += all;
+        __syncthreads();
+    }
+    if (tid == 0) plan[p.r.batch] = before;
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= p.r.batch; b += 32 * kSplitWarps) p.plan[b] = plan[b];
+    const unsigned long long total = before;
+    if (total == 0) return;
+    const int teams = split_teams(total, p.max_teams, 2 * TEAM);
+    const int team = TEAM == 1 ? (int)blockIdx.x * kSplitWarps + warp : (int)blockIdx.x;
+    if (team >= teams) return;
+    const unsigned long long start = share_start(total, teams, team), end = share_start(total, teams, team + 1);
+    int b = 0, hi = p.r.batch;
+    while (hi - b > 1) {
+        const int mid = (b + hi) / 2;
+        if (plan[mid] <= start) b = mid; else hi = mid;
+    }
+    const uint2* qf = qf_all + warp * S::QWORDS;
+    const float* qscale = qs_all[warp];
+    unsigned long long at = start;
+    while (at < end) {
+        while (plan[b + 1] <= at) ++b;
+        Block k;
+        k.b = b;
+        k.s = paged_seq(p.r, p.c.pt_stride, b, false);
+        const int blocks = split_blocks(p, k.s.n);
+        const PagedSpan span = paged_span(p, k.s.len - k.s.n, k.s.len - 1);
+        const int count = max(1, span.count);
+        const unsigned rest = (unsigned)(at - plan[b]), item = rest / (unsigned)count;
+        const int v0 = (int)(rest % (unsigned)count);
+        const unsigned long long left = end - at;
+        const int v1 = left < (unsigned long long)(count - v0) ? v0 + (int)left : count;
+        k.kvh = (int)item / blocks;
+        k.first = (int)item % blocks * 8;
+        k.count = min(8, k.s.n * p.group - k.first);
+        __syncwarp();
+        pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
+        __syncwarp();
+        float acc[HD / 16][4], m[2], l[2];
+        walk_pages<KVT, RT, HD>(p, k, span, v0 + (TEAM > 1 ? warp : 0), min(v1, span.count), TEAM, qf, qscale, acc, m, l);
+        const bool whole = v0 == 0 && v1 == count;
+        float* part = p.part + ((size_t)team * 2 + (at == start ? 0 : 1)) * S::PART;
+        if constexpr (TEAM == 1) {
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int i = 2 * j + c;
+                if (i >= k.count) continue;
+                if (whole) {
+                    int row, h, pos;
+                    block_row(p, k, i, row, h, pos);
+#pragma unroll
+                    for (int t = 0; t < HD / 16; ++t) odd |= put_pair<RT, HD>(p, row, h, pos, S::F::vdim(t, g), acc[t][c], acc[t][2 + c], l[c]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(part + i * S::W + S::F::vdim(t, g)) = make_float2(acc[t][c], acc[t][2 + c]);
+                    if (g == 0) { part[i * S::W + HD] = m[c]; part[i * S::W + HD + 1] = l[c]; }
+                }
+            }
+            if (__any_sync(0xffffffffu, odd)) {
+                for (int i = 0; i < k.count; ++i) {
+                    int row, h, pos;
+                    block_row(p, k, i, row, h, pos);
+                    careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
+                }
+            }
+        } else {
+            float* mine = red + warp * S::PART;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int i = 2 * j + c;
+#pragma unroll
+                for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(mine + i * S::W + S::F::vdim(t, g)) = make_float2(acc[t][c], acc[t][2 + c]);
+                if (g == 0) { mine[i * S::W + HD] = m[c]; mine[i * S::W + HD + 1] = l[c]; }
+            }
+            __syncthreads();
+            // a warp per row: the team's warps' results together
+            bool odd = false;
+            const int i = warp;
+            if (i < k.count) {
+                float mx = -INFINITY, lt = 0.f;
+#pragma unroll
+                for (int w = 0; w < kSplitWarps; ++w) mx = fmaxf(mx, red[w * S::PART + i * S::W + HD]);
+                const float ref = mx == -INFINITY ? 0.f : mx;
+                float2 o[HD / 64];
+#pragma unroll
+                for (int e = 0; e < HD / 64; ++e) o[e] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kSplitWarps; ++w) {
+                    const float* r = red + w * S::PART + i * S::W;
+                    const float f = ex2(r[HD] - ref);
+                    lt = fmaf(r[HD + 1], f, lt);
+#pragma unroll
+                    for (int e = 0; e < HD / 64; ++e) {
+                        const float2 x = *reinterpret_cast<const float2*>(r + e * 64 + lane * 2);
+                        o[e].x = fmaf(x.x, f, o[e].x);
+                        o[e].y = fmaf(x.y, f, o[e].y);
+                    }
+                }
+                int row, h, pos;
+                block_row(p, k, i, row, h, pos);
+#pragma unroll
+                for (int e = 0; e < HD / 64; ++e) {
+                    if (whole) odd |= put_pair<RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
+                    else *reinterpret_cast<float2*>(part + i * S::W + e * 64 + lane * 2) = o[e];
+                }
+                if (!whole && lane == 0) { part[i * S::W + HD] = mx; part[i * S::W + HD + 1] = lt; }
+                if (__any_sync(0xffffffffu, odd)) careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
+            }
+            __syncthreads();
+        }
+        at += (unsigned)(v1 - v0);
+    }
+}
+
+// Joins the partial results of the items that a share's end goes through: `WPR` warps per row, a CTA for kSplitWarps / WPR rows of an item.
+template <typename KVT, typename RT, int HD, int TEAM>
+__global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __grid_constant__ AttnPagedParams p, int max_blocks) {
+    using S = SplitShape<KVT, RT, HD>;
+    constexpr int WPR = TEAM == 1 ? 1 : kSplitWarps;
+    __shared__ float red[kSplitWarps][HD + 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = max_blocks * p.c.kv_heads, b = (int)blockIdx.x / per, item = (int)blockIdx.x % per;
+    const int i = WPR == 1 ? warp : (int)blockIdx.y;
+    Block k;
+    k.b = b;
+    k.s = paged_seq(p.r, p.c.pt_stride, b, false);
+    const int blocks = split_blocks(p, k.s.n);
+    pdl_wait();
+    if (item >= blocks * p.c.kv_heads) return;
+    k.kvh = item / blocks;
+    k.first = item % blocks * 8;
+    k.count = min(8, k.s.n * p.group - k.first);
+    if (i >= k.count) return;
+    const int count = max(1, paged_span(p, k.s.len - k.s.n, k.s.len - 1).count);
+    const unsigned long long total = __ldcg(p.plan + p.r.batch), o0 = __ldcg(p.plan + b) + (unsigned long long)item * count, o1 = o0 + count;
+    const int teams = split_teams(total, p.max_teams, 2 * TEAM);
+    // the team that holds page x: the last one that starts at or before it, x * teams / total or the next one
+    auto holder = [&](unsigned long long x) {
+        int t = (int)(x * (unsigned)teams / total);
+        while (t + 1 < teams && share_start(total, teams, t + 1) <= x) ++t;
+        return t;
+    };
+    const int t0 = holder(o0), t1 = holder(o1 - 1);
+    if (t0 == t1) return;                        // one team held it all and wrote the result
+    const int slot0 = share_start(total, teams, t0) == o0 ? 0 : 1;
+    auto part_of = [&](int t) { return p.part + ((size_t)t * 2 + (t == t0 ? slot0 : 0)) * S::PART + i * S::W; };
+    float mx = -INFINITY;
+    for (int t = t0 + lane; t <= t1; t += 32) mx = fmaxf(mx, __ldcg(part_of(t) + HD));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float2 o[HD / 64];
+    float lt = 0.f;
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) o[e] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int t = t0 + (WPR == 1 ? 0 : warp); t <= t1; t += WPR) {
+        const float* r = part_of(t);
+        const float f = ex2(__ldcg(r + HD) - ref);
+        lt = fmaf(__ldcg(r + HD + 1), f, lt);
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(r + e * 64 + lane * 2));
+            o[e].x = fmaf(x.x, f, o[e].x);
+            o[e].y = fmaf(x.y, f, o[e].y);
+        }
+    }
+    if constexpr (WPR > 1) {
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) *reinterpret_cast<float2*>(&red[warp][e * 64 + lane * 2]) = o[e];
+        if (lane == 0) red[warp][HD] = lt;
+        __syncthreads();
+        if (warp > 0) return;
+        lt = 0.f;
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) o[e] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) {
+            lt += red[w][HD];
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) {
+                o[e].x += red[w][e * 64 + lane * 2];
+                o[e].y += red[w][e * 64 + lane * 2 + 1];
+            }
+        }
+    }
+    int row, h, pos;
+    block_row(p, k, i, row, h, pos);
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) odd |= put_pair<RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
+    if (__any_sync(0xffffffffu, odd)) careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
+}
+
+// ---- more rows: a CTA per block of eight rows of a K/V head, its warps through the pages in turn ------------------------------
+template <typename KVT, typename RT, int HD>
+__global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const __grid_constant__ AttnPagedParams p) {
+    using S = SplitShape<KVT, RT, HD>;
+    extern __shared__ __align__(16) unsigned char sm[];
+    uint2* qf = reinterpret_cast<uint2*>(sm);
+    float* red = reinterpret_cast<float*>(sm + (size_t)S::QWORDS * 8);
+    __shared__ float qscale[8];
+    __shared__ int found[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
+    // which sequence's block this is: blocks of those with more than kSplitRows rows, one after another
+    if (warp == 0) {
+        int want = (int)(gridDim.x - 1 - blockIdx.x), at = -1;      // later rows, which see more, first
+        for (int b0 = 0; b0 < p.r.batch && at < 0; b0 += 32) {
+            const int b = b0 + lane;
+            int n = 0;
+            if (b < p.r.batch) {
+                const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0 && blockIdx.y == 0);
+                const long long rows = (long long)s.n * p.group;
+                n = rows > kSplitRows ? (int)((rows + 7) / 8) : 0;
+            }
+            int x = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned has = __ballot_sync(0xffffffffu, want < x);
+            if (has) {
+                const int src = __ffs(has) - 1;
+                const int before = __shfl_sync(0xffffffffu, x - n, src);
+                at = b0 + src;
+                want -= before;
+            } else {
+                want -= __shfl_sync(0xffffffffu, x, 31);
+            }
+        }
+        if (lane == 0) { found[0] = at; found[1] = want; }
+    }
+    __syncthreads();
+    if (found[0] < 0) return;
+    Block k;
+    k.b = found[0];
+    k.s = paged_seq(p.r, p.c.pt_stride, k.b, false);
+    k.kvh = blockIdx.y;
+    k.first = found[1] * 8;
+    k.count = min(8, k.s.n * p.group - k.first);
+    const int pos0 = k.s.len - k.s.n;
+    const PagedSpan span = paged_span(p, pos0 + k.first / p.group, pos0 + (k.first + k.count - 1) / p.group);
+    if (warp == 0) pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, qf, qscale, lane);
+    __syncthreads();
+    float acc[HD / 16][4], m[2], l[2];
+    walk_pages<KVT, RT, HD>(p, k, span, warp, span.count, kSplitWarps, qf, qscale, acc, m, l);
+    float* mine = red + warp * S::PART;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int i = 2 * j + c;
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(mine + i * S::W + S::F::vdim(t, g)) = make_float2(acc[t][c], acc[t][2 + c]);
+        if (g == 0) { mine[i * S::W + HD] = m[c]; mine[i * S::W + HD + 1] = l[c]; }
+    }
+    __syncthreads();
+    const int i = warp;
+    if (i >= k.count) return;
+    float mx = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) mx = fmaxf(mx, red[w * S::PART + i * S::W + HD]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float2 o[HD / 64];
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) o[e] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+        const float* r = red + w * S::PART + i * S::W;
+        const float f = ex2(r[HD] - ref);
+        lt = fmaf(r[HD + 1], f, lt);
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) {
+            const float2 x = *reinterpret_cast<const float2*>(r + e * 64 + lane * 2);
+            o[e].x = fmaf(x.x, f, o[e].x);
+            o[e].y = fmaf(x.y, f, o[e].y);
+        }
+    }
+    int row, h, pos;
+    block_row(p, k, i, row, h, pos);
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) odd |= put_pair<RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
+    if (__any_sync(0xffffffffu, odd)) careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
+}
+
+template <typename... KArgs>
+cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t st, KArgs... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename KVT, typename RT, int HD, int TEAM>
+cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
+    using S = SplitShape<KVT, RT, HD>;
+    const size_t smem = (size_t)kSplitWarps * S::QWORDS * 8 + (TEAM > 1 ? (size_t)kSplitWarps * S::PART * 4 : 0) + ((size_t)p.r.batch + 1) * 8;
+    cudaError_t e = cudaFuncSetAttribute(attn_split_kernel<KVT, RT, HD, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (e != cudaSuccess) return e;
+    const int ctas = 2 * sm_count;
+    p.max_teams = TEAM == 1 ? ctas * kSplitWarps : ctas;
+    attn_split_kernel<KVT, RT, HD, TEAM><<<ctas, 32 * kSplitWarps, smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const int blocks = p.r.row_start ? kSplitRows / 8 : 1;
+    const int rows = p.r.row_start ? 8 : std::min(8, p.group);
+    return launch_after(attn_join_kernel<KVT, RT, HD, TEAM>, dim3(p.r.batch * p.c.kv_heads * blocks, TEAM == 1 ? 1 : rows), 32 * kSplitWarps, st, p, blocks);
+}
+
+template <typename KVT, typename RT, int HD>
+cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) {
+    using S = SplitShape<KVT, RT, HD>;
+    // Each warp alone where there are sequences and heads enough to give most of them whole items: nothing to put together in a CTA.
+    const long long items = (long long)p.r.batch * p.c.kv_heads;
+    cudaError_t e = items >= 4LL * sm_count ? split_launch<KVT, RT, HD, 1>(p, sm_count, st) : split_launch<KVT, RT, HD, kSplitWarps>(p, sm_count, st);
+    if (e != cudaSuccess || !p.r.row_start) return e;
+    const long long most = p.r.max_rows > 0 ? std::min(p.r.max_rows, p.r.rows) : p.r.rows;
+    if (most * p.group <= kSplitRows) return e;
+    const size_t smem = (size_t)S::QWORDS * 8 + (size_t)kSplitWarps * S::PART * 4;
+    e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    if (e != cudaSuccess) return e;
+    const long long blocks = (long long)p.r.rows * p.group / 8 + p.r.batch;
+    attn_blocks_kernel<KVT, RT, HD><<<dim3((unsigned)blocks, p.c.kv_heads), 32 * kSplitWarps, smem, st>>>(p);
+    return cudaGetLastError();
 }
 
 template <typename KVT, typename RT>
-cudaError_t rows_launch(const AttnPagedParams& p, int hd, cudaStream_t st) {
-    const unsigned ctas = (unsigned)(((long long)p.r.rows * p.heads + 7) / 8);
-    if (hd == 64) attn_paged_rows_kernel<KVT, RT, 64><<<ctas, 256, 0, st>>>(p);
-    else attn_paged_rows_kernel<KVT, RT, 128><<<ctas, 256, 0, st>>>(p);
-    return cudaGetLastError();
+cudaError_t launch_types(const AttnPagedParams& p, int hd, int sm_count, cudaStream_t st) {
+    return hd == 64 ? launch_one<KVT, RT, 64>(p, sm_count, st) : launch_one<KVT, RT, 128>(p, sm_count, st);
 }
 
 }  // namespace
 
-size_t attn_paged_part_bytes(int sm_count) { return (size_t)sm_count * 16 * 2 * 8 * 130 * 4; }
+size_t attn_paged_part_bytes(int sm_count) { return (size_t)sm_count * 2 * kSplitWarps * 2 * split_part_floats(128) * 4; }
 
 cudaError_t attn_paged_launch(const AttnPagedParams& p, int dtype, int row_dtype, int head_dim, int sm_count, cudaStream_t st) {
     const bool f = row_dtype == MLB_DT_F32;
-    if (dtype == MLB_DT_F32) return f ? rows_launch<float, float>(p, head_dim, st) : rows_launch<float, bf16_t>(p, head_dim, st);
-    if (dtype == MLB_DT_BF16) return f ? rows_launch<bf16_t, float>(p, head_dim, st) : rows_launch<bf16_t, bf16_t>(p, head_dim, st);
-    return f ? rows_launch<fp4_t, float>(p, head_dim, st) : rows_launch<fp4_t, bf16_t>(p, head_dim, st);
+    if (dtype == MLB_DT_F32) return f ? launch_types<float, float>(p, head_dim, sm_count, st) : launch_types<float, bf16_t>(p, head_dim, sm_count, st);
+    if (dtype == MLB_DT_BF16) return f ? launch_types<bf16_t, float>(p, head_dim, sm_count, st) : launch_types<bf16_t, bf16_t>(p, head_dim, sm_count, st);
+    return f ? launch_types<fp4_t, float>(p, head_dim, sm_count, st) : launch_types<fp4_t, bf16_t>(p, head_dim, sm_count, st);
 }
 
 }  // namespace mlb
