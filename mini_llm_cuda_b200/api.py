@@ -416,6 +416,23 @@ _ROW_DTYPES = {"torch.float32": DT_F32, "torch.bfloat16": DT_BF16}
 _CACHE_DTYPES = {**_ROW_DTYPES, "torch.uint8": DT_FP4}
 
 
+_dtype_seen = {}
+
+
+def _row_dtype(dtype):
+    """mlb_dtype of a torch dtype that rows may have, else None; the text of a dtype is made once."""
+    if dtype not in _dtype_seen:
+        _dtype_seen[dtype] = _ROW_DTYPES.get(str(dtype))
+    return _dtype_seen[dtype]
+
+
+def _one_device(tensors) -> int:
+    devices = {t.get_device() for t in tensors}
+    if len(devices) != 1:
+        raise ValueError(f"tensors on several devices: {sorted(devices)}")
+    return devices.pop()
+
+
 def _dense(x, what: str, dtypes, shape=None):
     if str(x.dtype) not in dtypes:
         raise ValueError(f"{what} is {x.dtype}: expected one of {', '.join(dtypes)}")
@@ -446,7 +463,9 @@ class PagedKV:
             for x, what in ((kscale, "kscale"), (vscale, "vscale")):
                 _dense(x, what, ("torch.float8_e4m3fn", "torch.uint8"), (pages, self.kv_heads, 16, self.head_dim // 16))
         self.batch = page_table.shape[0]
+        self.width = self.kv_heads * self.head_dim
         self.tensors = [t for t in (kpool, vpool, page_table, kscale, vscale) if t is not None]
+        self.device = _one_device(self.tensors)
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         self.struct = PagedKvStruct(ptr(kpool), ptr(vpool), ptr(kscale), ptr(vscale), ptr(page_table), page_table.shape[1], pages,
                                     self.kv_heads, self.head_dim, self.dtype, k_scale, v_scale)
@@ -463,6 +482,7 @@ class NewRows:
         if row_start is not None:
             _dense(row_start, "row_start", ("torch.int32",), (self.batch + 1,))
         self.tensors = [t for t in (kv_lens, row_start) if t is not None]
+        self.device = _one_device(self.tensors)
         self.struct = NewRowsStruct(row_start.data_ptr() if row_start is not None else None, kv_lens.data_ptr(), self.batch, self.rows, max_rows)
         self.ref = C.byref(self.struct)
 
@@ -479,53 +499,53 @@ class Ops:
         L = lib()
         self._append, self._read, self._attn = L.mlb_op_kv_append, L.mlb_op_kv_read, L.mlb_op_attn_paged
 
-    def _rows(self, x, what: str, rows: NewRows, width: int, dtype=None):
-        """(pointer, stride) of a row tensor."""
-        if dtype is not None and x.dtype != dtype:
-            raise ValueError(f"{what} is {x.dtype}: expected {dtype}")
+    def _rows(self, x, what: str, rows: NewRows, width: int, dtype):
+        """(pointer, stride) of a row tensor; called for every tensor of every call, so the common case is checked first."""
         shape = x.shape
-        if x.get_device() != self.device:
-            raise ValueError(f"{what} is not on CUDA device {self.device}")
-        inner = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else -1
-        if shape[0] != rows.rows or inner != width or x.stride(-1) != 1 or (len(shape) == 3 and x.stride(1) != shape[2]):
-            raise ValueError(f"{what} must be [{rows.rows}][{width}], dense within a row")
+        if x.dtype is not dtype or x.get_device() != self.device or len(shape) != 2 or shape[0] != rows.rows or shape[1] != width or \
+                (x.stride(1) != 1 and width > 1):
+            if x.dtype is not dtype:
+                raise ValueError(f"{what} is {x.dtype}: expected {dtype}")
+            if x.get_device() != self.device:
+                raise ValueError(f"{what} is not on CUDA device {self.device}")
+            if len(shape) != 3 or shape[0] != rows.rows or shape[1] * shape[2] != width or x.stride(2) != 1 or x.stride(1) != shape[2]:
+                raise ValueError(f"{what} must be [{rows.rows}][{width}], dense within a row")
         return x.data_ptr(), x.stride(0)
 
     def _check(self, cache: PagedKV, rows: NewRows, x, what: str) -> int:
         if cache.batch < rows.batch:
             raise ValueError(f"the page table has {cache.batch} rows, the call {rows.batch} sequences")
-        for t in cache.tensors + rows.tensors:
-            if t.get_device() != self.device:
-                raise ValueError(f"the cache and its rows must be on CUDA device {self.device}")
-        dt = _ROW_DTYPES.get(str(x.dtype))
+        if cache.device != self.device or rows.device != self.device:
+            raise ValueError(f"the cache and its rows must be on CUDA device {self.device}")
+        dt = _row_dtype(x.dtype)
         if dt is None:
             raise ValueError(f"{what} is {x.dtype}: expected float32 or bfloat16")
         return dt
 
     def kv_append(self, cache: PagedKV, rows: NewRows, k, v, rope=None, q=None, q_out=None, heads: int = 0, stream: int = 0):
         """Rotates k (and q into q_out, which may be q) by the rows' positions and writes k and v to their pages."""
+        dtype = k.dtype
         dt = self._check(cache, rows, k, "k")
-        width = cache.kv_heads * cache.head_dim
-        kp, ks = self._rows(k, "k", rows, width)
-        vp_, vs = self._rows(v, "v", rows, width, k.dtype)
+        kp, ks = self._rows(k, "k", rows, cache.width, dtype)
+        vp_, vs = self._rows(v, "v", rows, cache.width, dtype)
         qp, qs, op, os_ = None, 0, None, 0
         if q is not None:
-            qp, qs = self._rows(q, "q", rows, heads * cache.head_dim, k.dtype)
-            op, os_ = self._rows(q_out, "q_out", rows, heads * cache.head_dim, k.dtype)
+            qp, qs = self._rows(q, "q", rows, heads * cache.head_dim, dtype)
+            op, os_ = self._rows(q_out, "q_out", rows, heads * cache.head_dim, dtype)
         rp, rl = None, 0
         if rope is not None:
-            _dense(rope, "rope", ("torch.float32",), (rope.shape[0], cache.head_dim))
-            if rope.get_device() != self.device:
-                raise ValueError(f"rope is not on CUDA device {self.device}")
-            rp, rl = rope.data_ptr(), rope.shape[0]
+            shape = rope.shape
+            if _row_dtype(rope.dtype) != DT_F32 or len(shape) != 2 or shape[1] != cache.head_dim or not rope.is_contiguous() or \
+                    rope.get_device() != self.device:
+                raise ValueError(f"rope must be a contiguous fp32 [positions][{cache.head_dim}] on CUDA device {self.device}")
+            rp, rl = rope.data_ptr(), shape[0]
         check(self._append(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, rp, rl, qp, qs, op, os_, heads, stream))
 
     def kv_read(self, cache: PagedKV, rows: NewRows, k_out, v_out, stream: int = 0):
         """The rows' cached keys and values, as values."""
         dt = self._check(cache, rows, k_out, "k_out")
-        width = cache.kv_heads * cache.head_dim
-        kp, ks = self._rows(k_out, "k_out", rows, width)
-        vp_, vs = self._rows(v_out, "v_out", rows, width, k_out.dtype)
+        kp, ks = self._rows(k_out, "k_out", rows, cache.width, k_out.dtype)
+        vp_, vs = self._rows(v_out, "v_out", rows, cache.width, k_out.dtype)
         check(self._read(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, stream))
 
     def attn_paged(self, cache: PagedKV, rows: NewRows, q, out, heads: int, gate=None, scale: float = 0.0, window: int = 0, sinks: int = 0,
@@ -533,12 +553,13 @@ class Ops:
         """Causal attention of the rows, optionally within a window and to the first `sinks` positions (mlb_op_attn_paged)."""
         dt = self._check(cache, rows, q, "q")
         width = heads * cache.head_dim
-        qp, qs = self._rows(q, "q", rows, width)
+        qp, qs = self._rows(q, "q", rows, width, q.dtype)
         op, os_ = self._rows(out, "out", rows, width, q.dtype)
         gp = None
         if gate is not None:
-            _dense(gate, "gate", ("torch.float32",))
-            gp, gs = self._rows(gate, "gate", rows, width)
+            if _row_dtype(gate.dtype) != DT_F32 or not gate.is_contiguous():
+                raise ValueError("gate must be a contiguous fp32 tensor")
+            gp, _ = self._rows(gate, "gate", rows, width, gate.dtype)
         check(self._attn(self._h, cache.ref, rows.ref, dt, qp, qs, gp, op, os_, heads, scale, window, sinks, stream))
 
     def status(self, stream: int = 0):

@@ -1,5 +1,6 @@
 // Operators over a caller's paged K/V cache: the handle, the rotating append, the read, and the entry point of the attention (its
 // kernels are in paged_attn.cu).
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -413,7 +414,8 @@ extern "C" int mlb_op_attn_paged(mlb_ops* o, const mlb_paged_kv* kv, const mlb_n
     p.q = q; p.q_stride = q_stride; p.gate = gate_or_null; p.out = out; p.out_stride = out_stride;
     p.heads = heads; p.group = heads / kv->kv_heads;
     p.scale = scale != 0.f ? scale : 1.f / std::sqrt((float)kv->head_dim);
-    p.window = window; p.sinks = sinks;
+    p.window = std::min(window, 1 << 30);        // no position reaches that far (pt_stride), and differences stay within 32 bits
+    p.sinks = std::min(sinks, 1 << 30);
     p.plan = reinterpret_cast<unsigned long long*>(o->mem + kOpsErrBytes);
     p.part = reinterpret_cast<float*>(o->mem + kOpsErrBytes + kOpsPlanBytes);
     OnDevice on(o->device);

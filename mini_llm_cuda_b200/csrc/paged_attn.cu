@@ -3,79 +3,12 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "paged.cuh"
+#include "paged_prompt.h"
+#include "paged_row.cuh"
 
 namespace mlb {
 
 namespace {
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// ---- one row, one head, by one warp, straight from the formula --------------------------------------------------------
-// A product with a probability that is not of the row's own positions does not happen here, so infinities and NaN outside of them cannot
-// reach the row, and an infinite score or value gives what the formula gives. The matrix-core kernels redo a row here whose result is
-// not finite: there a probability of 0 times an infinity, or a piece of an infinite number, is a NaN.
-template <typename KVT, typename RT, int HD>
-__device__ __noinline__ void careful_row(const AttnPagedParams& p, int b, int pos, int row, int h) {
-    constexpr int E = HD / 32;                   // dims of a lane
-    const int lane = threadIdx.x & 31, kvh = h / p.group;
-    float q[E], o[E], top = -INFINITY, sum = 0.f;
-    const RT* qp = static_cast<const RT*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = Elem<RT>::get(qp, e);
-        o[e] = 0.f;
-    }
-    auto get = [&](bool k, size_t at, float (&x)[E]) {      // this lane's dims of pool row `at`
-        if constexpr (sizeof(KVT) == 1) {
-            const unsigned char* codes = static_cast<const unsigned char*>(k ? p.c.kpool : p.c.vpool) + at * (HD / 2) + lane * E / 2;
-            const float s = e4m3_to_f32((k ? p.c.kscale : p.c.vscale)[at * (HD / 16) + lane * E / 16]);
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                x[e] = e2m1_value(codes[e / 2] & 15) * s;
-                x[e + 1] = e2m1_value(codes[e / 2] >> 4) * s;
-            }
-        } else {
-            const KVT* src = static_cast<const KVT*>(k ? p.c.kpool : p.c.vpool) + at * HD + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = Elem<KVT>::get(src, e);
-        }
-    };
-    const PagedSpan span = paged_span(p, pos, pos);
-    const float scale = p.scale * p.c.k_scale;
-    bool any = false;
-    for (int v = 0; v < span.count; ++v) {
-        const int pg = span.page(v), id = paged_page(p.c, p.r.err, b, pg, 0);
-        const size_t base = ((size_t)id * p.c.kv_heads + kvh) * kKvBlock;
-        for (int j = 0; j < kKvBlock; ++j) {
-            if (!paged_sees(p, pos, pg * kKvBlock + j)) continue;
-            float x[E], s = 0.f;
-            get(true, base + j, x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) s = fmaf(q[e], x[e], s);
-            s = warp_sum(s) * scale;
-            any = true;
-            const float mn = fmaxf(top, s), ref = mn == -INFINITY ? 0.f : mn;
-            const float f = top == mn ? 1.f : expf(top - ref), w = expf(s - ref);
-            top = mn;
-            sum = sum * f + w;
-            get(false, base + j, x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[e], o[e] * f);
-        }
-    }
-    RT* op = static_cast<RT*>(p.out) + (size_t)row * p.out_stride + (size_t)h * HD + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        float y = any ? o[e] / sum * p.c.v_scale : 0.f;
-        if (p.gate) y *= p.gate[(size_t)row * p.heads * HD + (size_t)h * HD + lane * E + e];
-        Elem<RT>::put(op, e, y);
-    }
-}
 
 // ---- blocks of up to eight rows on matrix cores -------------------------------------------------------------------------
 // A warp takes pages of 16 positions of one K/V head for a block of up to 8 rows (new tokens x the query heads of the K/V head):
@@ -509,8 +442,6 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
 // head, block of rows) are laid end to end and cut into as many equal shares as there are teams (a CTA's warps together, or each warp alone),
 // and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Sequences of more than
 // kSplitRows (token, head) pairs are left to the kernels for prompts.
-constexpr int kSplitRows = 32;
-
 // (sequences, pages of their items before them) -> plan in shared memory; returns the total
 __device__ __forceinline__ int split_blocks(const AttnPagedParams& p, int n) {
     const long long rows = (long long)n * p.group;
@@ -887,6 +818,7 @@ cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) 
     if (e != cudaSuccess || !p.r.row_start) return e;
     const long long most = p.r.max_rows > 0 ? std::min(p.r.max_rows, p.r.rows) : p.r.rows;
     if (most * p.group <= kSplitRows) return e;
+    if constexpr (sizeof(KVT) == 2 && sizeof(RT) == 2) return attn_prompt_launch(p, HD, st);
     const size_t smem = (size_t)S::QWORDS * 8 + (size_t)kSplitWarps * S::PART * 4;
     e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e != cudaSuccess) return e;

@@ -1,0 +1,428 @@
+// Paged attention of many rows of a sequence (prompts and chunks of prompts) on the 5th-generation tensor cores.
+//
+// A CTA takes 256 consecutive (token, query head) rows of one K/V head, as two tiles of 128, through the pages that any of them sees, 128
+// positions at a time:  S = Q K^T, P = exp2(S - m), O += P V. S (fp32) and O lie in tensor memory, P as bf16 over the columns of its S, so
+// that it is the MMA's A operand from there. One warp brings K and V (TMA, a page at a time: 16 rows of 128-byte swizzled halves), one
+// thread issues the MMAs, and four warps per tile take a row per thread: maximum, exponentials, sum, without any exchange between threads.
+// The two tiles alternate on the tensor core: while one's products run, the other's exponentials are taken.
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the reference of its weights was set.
+// Positions that no row of the CTA sees (behind the last one, between the first positions and the window) are zeros in V: 0 times what
+// may lie there could be no number. A row whose result is not finite is done again from the formula (careful_row).
+#include <cstring>
+
+#include "paged_prompt.h"
+#include "paged_row.cuh"
+#include "tc_host.h"
+
+namespace mlb {
+
+namespace {
+
+constexpr int kPpTiles = 2;
+constexpr int kPpKeys = 128;                     // positions of a step
+constexpr int kPpPages = kPpKeys / kKvBlock;
+constexpr int kPpThreads = 128 * kPpTiles + 64;  // softmax warps, then the loader's and the issuer's
+constexpr float kPpLazy = 8.f;
+constexpr uint32_t kPpSpin = 1u << 24;
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+        "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+        "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+        : "memory");
+}
+// The registers of loads that tmem_ld_wait() has waited for: no use of them is moved before it
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                   "+r"(r[31]));
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// B operand whose N runs along the 128-byte rows (V: a row is a position, the dims are N): 64 dims a row, 128-byte swizzle, groups of
+// eight positions 1024 bytes apart, the next 64 dims `next` bytes on.
+__device__ __forceinline__ uint64_t umma_desc_rows_are_k(uint32_t smem_addr, uint32_t next) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(next >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <int HD>
+struct PromptSmem {
+    static constexpr uint32_t kQ = 128 * HD * 2, kKV = kPpKeys * HD * 2, kHalf = 128 * 128;      // bytes of a tile; of 64 dims of one
+    static constexpr uint32_t q = 0, k = kPpTiles * kQ, v = k + 2 * kKV, bars = v + 2 * kKV, total = bars + 256;
+};
+enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_O = 13, PB_COUNT = 15 };
+
+template <int HD>
+__global__ void __launch_bounds__(kPpThreads, 1)
+    attn_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnPagedParams p) {
+    using L = PromptSmem<HD>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t sm0 = smem_u32(sm), bar0 = sm0 + L::bars;
+    auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+    __shared__ uint32_t tmem_base;
+    __shared__ int found[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kLoader = 4 * kPpTiles, kIssuer = kLoader + 1;
+
+    if (warp == kLoader) {
+        // which sequence's rows these are: those of sequences with more than kSplitRows, 256 at a time, later rows (which see more) first
+        int want = (int)(gridDim.x - 1 - blockIdx.x), at = -1;
+        for (int b0 = 0; b0 < p.r.batch && at < 0; b0 += 32) {
+            const int b = b0 + lane;
+            int n = 0;
+            if (b < p.r.batch) {
+                const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0 && blockIdx.y == 0);
+                const long long rows = (long long)s.n * p.group;
+                n = rows > kSplitRows ? (int)((rows + 128 * kPpTiles - 1) / (128 * kPpTiles)) : 0;
+            }
+            int x = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned has = __ballot_sync(0xffffffffu, want < x);
+            if (has) {
+                const int src = __ffs(has) - 1;
+                at = b0 + src;
+                want -= __shfl_sync(0xffffffffu, x - n, src);
+            } else {
+                want -= __shfl_sync(0xffffffffu, x, 31);
+            }
+        }
+        if (lane == 0) {
+            found[0] = at;
+            found[1] = want;
+            for (int i = 0; i < PB_COUNT; ++i) mbar_init(bar(i), i == PB_Q ? 128 * kPpTiles : i == PB_P || i == PB_P + 1 ? 128 : 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    __syncthreads();
+    if (found[0] < 0) return;                    // (uniform)
+    if (warp == kIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;             // S0 | S1 | O0 | O1, 128 columns each
+    const int b = found[0], kvh = blockIdx.y, first = found[1] * 128 * kPpTiles;
+    const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, false);
+    const int count = min(128 * kPpTiles, s.n * p.group - first), tiles = count > 128 ? 2 : 1;
+    const int pos0 = s.len - s.n, low = pos0 + first / p.group, high = pos0 + (first + count - 1) / p.group;
+    const PagedSpan span = paged_span(p, low, high);
+    const int steps = (span.count + kPpPages - 1) / kPpPages;
+    auto wait = [&](int i, uint32_t parity) {
+        if (mbar_wait_bounded(bar(i), parity, kPpSpin, 0)) return true;
+        atomicExch(p.r.err, PG_WAIT);
+        return false;
+    };
+
+    if (warp == kLoader) {
+        bool good = true;
+        for (int j = 0; j < steps && good; ++j) {
+            const int st = j & 1;
+            const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+            const int v = j * kPpPages + (lane & 7), pg = v < span.count ? span.page(v) : 0;
+            const bool held = lane < kPpPages && v < span.count;
+            const int row0 = held ? (int)(((long long)paged_page(p.c, p.r.err, b, pg, 0) * p.c.kv_heads + kvh) * kKvBlock) : 0;
+            const int key0 = pg * kKvBlock;
+            // a page with positions that no row sees is copied by the warp, with zeros in their place
+            const bool partly = key0 + kKvBlock - 1 > high || (p.window > 0 && key0 <= low - p.window && key0 + kKvBlock > p.sinks);
+            const unsigned all = __ballot_sync(0xffffffffu, held), by_hand = __ballot_sync(0xffffffffu, lane < kPpPages && (!held || partly));
+            good = __all_sync(0xffffffffu, wait(PB_KEMPTY + st, ph ^ 1u));
+            if (!good) break;
+            if (lane == 0) mbar_expect_tx(bar(PB_KFULL + st), (uint32_t)__popc(all) * kKvBlock * HD * 2);
+            __syncwarp();
+            if (held) {
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h)
+                    tma_load_2d(sm0 + L::k + st * L::kKV + h * L::kHalf + lane * 2048, &tmK, h * 64, row0, bar(PB_KFULL + st));
+            }
+            good = __all_sync(0xffffffffu, wait(PB_VEMPTY + st, ph ^ 1u));
+            if (!good) break;
+            for (unsigned left = by_hand; left; left &= left - 1) {
+                const int i = __ffs(left) - 1, k0 = __shfl_sync(0xffffffffu, key0, i), r0 = __shfl_sync(0xffffffffu, row0, i);
+                const bool here = (all >> i) & 1u;
+                for (int e = lane; e < kKvBlock * HD / 8; e += 32) {
+                    const int row = e / (HD / 8), ch = e % (HD / 8), key = k0 + row, at = i * kKvBlock + row;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (here && key <= high && !(p.window > 0 && key <= low - p.window && key >= p.sinks))
+                        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16_t*>(p.c.vpool) + (size_t)(r0 + row) * HD) + ch);
+                    *reinterpret_cast<uint4*>(sm + L::v + st * L::kKV + ch / 8 * L::kHalf + at * 128 + ((ch % 8) ^ (at & 7)) * 16) = x;
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_expect_tx(bar(PB_VFULL + st), (uint32_t)(kPpPages - __popc(by_hand)) * kKvBlock * HD * 2);
+            __syncwarp();
+            if (held && !partly) {
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h)
+                    tma_load_2d(sm0 + L::v + st * L::kKV + h * L::kHalf + lane * 2048, &tmV, h * 64, row0, bar(PB_VFULL + st));
+            }
+        }
+    } else if (warp == kIssuer) {
+        if (lane == 0 && steps > 0) {
+            const uint32_t is = umma_idesc_bf16(128, kPpKeys), io = umma_idesc_bf16(128, HD) | (1u << 16);      // bit 16: N runs along B's rows
+            auto scores = [&](int t, int j) {
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint32_t off = (uint32_t)(ks / 4) * L::kHalf + (uint32_t)(ks % 4) * 32;
+                    umma_bf16(tmem + t * 128, umma_desc_sw128(sm0 + L::q + t * L::kQ + off), umma_desc_sw128(sm0 + L::k + (j & 1) * L::kKV + off), is, ks > 0);
+                }
+                umma_commit(bar(PB_S + t));
+            };
+            bool good = wait(PB_Q, 0) && wait(PB_KFULL, 0);
+            tc_fence_after();
+            if (good) {
+                for (int t = 0; t < tiles; ++t) scores(t, 0);
+                umma_commit(bar(PB_KEMPTY));
+            }
+            for (int j = 0; j < steps && good; ++j) {
+                const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+                for (int t = 0; t < tiles && good; ++t) {
+                    good = wait(PB_P + t, (uint32_t)j & 1u) && (t > 0 || wait(PB_VFULL + (j & 1), ph));
+                    if (!good) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < kPpKeys / 16; ++ks)
+                        umma_bf16_ta(tmem + (2 + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + (j & 1) * L::kKV + ks * 2048, L::kHalf), io,
+                                     j > 0 || ks > 0);
+                    if (t == tiles - 1) umma_commit(bar(PB_VEMPTY + (j & 1)));
+                    if (j + 1 < steps) {
+                        if (t == 0) {
+                            good = wait(PB_KFULL + ((j + 1) & 1), (((uint32_t)j + 1) >> 1) & 1u);
+                            if (!good) break;
+                            tc_fence_after();
+                        }
+                        scores(t, j + 1);
+                        if (t == tiles - 1) umma_commit(bar(PB_KEMPTY + ((j + 1) & 1)));
+                    } else {
+                        umma_commit(bar(PB_O + t));
+                    }
+                }
+            }
+        }
+    } else {
+        const int t = warp / 4, r = tid & 127, i = t * 128 + r;      // this thread's row of the CTA's
+        const bool in = i < count;
+        const int rr = first + (in ? i : 0), row = s.r0 + rr / p.group, h = kvh * p.group + rr % p.group;
+        const int pos = in ? pos0 + rr / p.group : high;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // the warp's 32 lanes of tensor memory
+        // the row's queries, K-major with the swizzle that the MMA expects; a negative scale turns their sign
+        const float scale = p.scale * p.c.k_scale * 1.4426950408889634f;
+        {
+            const bf16_t* q = static_cast<const bf16_t*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD;
+            const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+            const uint32_t turn = scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (in) {
+                    if (vec) {
+                        x = __ldg(reinterpret_cast<const uint4*>(q) + c);
+                    } else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = (uint32_t)__bfloat16_as_ushort(q[c * 8 + 2 * e]) | (uint32_t)__bfloat16_as_ushort(q[c * 8 + 2 * e + 1]) << 16;
+                        x = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    x.x ^= turn; x.y ^= turn; x.z ^= turn; x.w ^= turn;
+                }
+                *reinterpret_cast<uint4*>(sm + L::q + t * L::kQ + c / 8 * L::kHalf + r * 128 + ((c % 8) ^ (r & 7)) * 16) = x;
+            }
+            fence_async_smem();
+            mbar_arrive(bar(PB_Q));
+        }
+        const float c = fabsf(scale);
+        float m = -INFINITY, l = 0.f;
+        bool good = true;
+        if (t < tiles) {
+            const int wlow = __reduce_min_sync(0xffffffffu, pos), whigh = __reduce_max_sync(0xffffffffu, pos);
+            for (int j = 0; j < steps; ++j) {
+                good = __all_sync(0xffffffffu, wait(PB_S + t, (uint32_t)j & 1u));
+                if (!good) break;
+                tc_fence_after();
+                uint32_t x[4][32];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tmem_ld32(tmem + lanes + t * 128 + e * 32, x[e]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tmem_loaded(x[e]);
+                // positions that some row of the warp does not see
+                bool edge = (j + 1) * kPpPages > span.count;
+                if (!edge) {
+                    const int ka = span.page(j * kPpPages) * kKvBlock, kb = span.page(j * kPpPages + kPpPages - 1) * kKvBlock + kKvBlock - 1;
+                    edge = kb > wlow || (p.window > 0 && ka <= whigh - p.window && !(kb < p.sinks));
+                }
+                if (edge) {
+#pragma unroll
+                    for (int g = 0; g < kPpPages; ++g) {
+                        const int v = j * kPpPages + g, k0 = v < span.count ? span.page(v) * kKvBlock : 0x40000000;
+                        const int hi = pos - k0, lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) - k0, sk = p.sinks - k0;
+#pragma unroll
+                        for (int e = 0; e < kKvBlock; ++e) {
+                            const int at = g * kKvBlock + e;
+                            if (!(e <= hi && (e >= lo || e < sk))) x[at / 32][at % 32] = 0xff800000u;      // -inf
+                        }
+                    }
+                }
+                float top[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top[e] = __uint_as_float(x[0][e]);
+#pragma unroll
+                for (int at = 8; at < kPpKeys; ++at) top[at % 8] = fmaxf(top[at % 8], __uint_as_float(x[at / 32][at % 32]));
+                const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7]))) * c;
+                const bool moved = mx > m + kPpLazy;
+                if (__any_sync(0xffffffffu, moved)) {
+                    const float f = moved ? ex2(m - mx) : 1.f;
+                    if (moved) m = mx;
+                    l *= f;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int e = 0; e < HD / 32; ++e) {
+                            uint32_t o[32];
+                            tmem_ld32(tmem + lanes + (2 + t) * 128 + e * 32, o);
+                            tmem_ld_wait();
+                            tmem_loaded(o);
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                            tmem_st32(tmem + lanes + (2 + t) * 128 + e * 32, o);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) {
+                        const int at = half * 64 + 2 * u;
+                        const float a = ex2(fmaf(__uint_as_float(x[at / 32][at % 32]), c, -ref)), d = ex2(fmaf(__uint_as_float(x[at / 32][at % 32 + 1]), c, -ref));
+                        sum[u % 2 * 2] += a;
+                        sum[u % 2 * 2 + 1] += d;
+                        w[u] = f32x2_to_bf16(a, d);
+                    }
+                    tmem_st32(tmem + lanes + t * 128 + half * 32, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(bar(PB_P + t));
+            }
+            // results
+            if (steps > 0 && good) {
+                good = __all_sync(0xffffffffu, wait(PB_O + t, 0));
+                tc_fence_after();
+            }
+            if (good) {
+                const float inv = pos < 0 ? 0.f : p.c.v_scale / l;
+                bool odd = false;
+                bf16_t* out = static_cast<bf16_t*>(p.out) + (size_t)row * p.out_stride + (size_t)h * HD;
+                const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll 1
+                for (int e = 0; e < HD / 32; ++e) {
+                    uint32_t o[32];
+                    if (steps > 0) {
+                        tmem_ld32(tmem + lanes + (2 + t) * 128 + e * 32, o);
+                        tmem_ld_wait();
+                        tmem_loaded(o);
+                    }
+                    float y[32];
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) {
+                        y[u] = pos < 0 ? 0.f : __uint_as_float(o[u]) * inv;
+                        odd |= !(fabsf(y[u]) <= 3.4e38f);
+                    }
+                    if (p.gate && in) {
+                        const float* gp = p.gate + (size_t)row * p.heads * HD + (size_t)h * HD + e * 32;
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) y[u] *= gp[u];
+                    }
+                    if (in) {
+                        if (vec) {
+#pragma unroll
+                            for (int u = 0; u < 32; u += 8)
+                                *reinterpret_cast<uint4*>(out + e * 32 + u) = make_uint4(f32x2_to_bf16(y[u], y[u + 1]), f32x2_to_bf16(y[u + 2], y[u + 3]),
+                                                                                         f32x2_to_bf16(y[u + 4], y[u + 5]), f32x2_to_bf16(y[u + 6], y[u + 7]));
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) out[e * 32 + u] = __float2bfloat16_rn(y[u]);
+                        }
+                    }
+                }
+                for (unsigned again = __ballot_sync(0xffffffffu, odd && in); again; again &= again - 1) {
+                    const int src = __ffs(again) - 1;
+                    careful_row<bf16_t, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == kIssuer) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+template <int HD>
+cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st) {
+    alignas(64) CUtensorMap tk, tv;
+    const uint64_t rows = (uint64_t)p.c.num_pages * p.c.kv_heads * kKvBlock;
+    if (make_bf16_map(enc, &tk, p.c.kpool, rows, HD, kKvBlock) || make_bf16_map(enc, &tv, p.c.vpool, rows, HD, kKvBlock)) return cudaErrorInvalidValue;
+    const size_t smem = PromptSmem<HD>::total + 1024;
+    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles) + p.r.batch;
+    attn_prompt_kernel<HD><<<dim3((unsigned)tiles, p.c.kv_heads), kPpThreads, smem, st>>>(tk, tv, p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t attn_prompt_launch(const AttnPagedParams& p, int head_dim, cudaStream_t st) {
+    static const EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return cudaErrorNotSupported;
+    return head_dim == 64 ? launch<64>(enc, p, st) : launch<128>(enc, p, st);
+}
+
+}  // namespace mlb
