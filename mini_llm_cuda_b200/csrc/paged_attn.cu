@@ -818,7 +818,7 @@ cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) 
     if (e != cudaSuccess || !p.r.row_start) return e;
     const long long most = p.r.max_rows > 0 ? std::min(p.r.max_rows, p.r.rows) : p.r.rows;
     if (most * p.group <= kSplitRows) return e;
-    if constexpr (sizeof(KVT) == 2 && sizeof(RT) == 2) return attn_prompt_launch(p, HD, st);
+    if constexpr (sizeof(KVT) <= 2 && sizeof(RT) == 2) return attn_prompt_launch(p, sizeof(KVT) == 1 ? MLB_DT_FP4_E2M1 : MLB_DT_BF16, HD, st);
     const size_t smem = (size_t)S::QWORDS * 8 + (size_t)kSplitWarps * S::PART * 4;
     e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e != cudaSuccess) return e;

@@ -21,7 +21,8 @@ namespace {
 constexpr int kPpTiles = 2;
 constexpr int kPpKeys = 128;                     // positions of a step
 constexpr int kPpPages = kPpKeys / kKvBlock;
-constexpr int kPpThreads = 128 * kPpTiles + 64;  // softmax warps, then the loader's and the issuer's
+template <typename KVT> constexpr int kPpLoaders = sizeof(KVT) == 1 ? 4 : 1;                             // warps that bring K and V
+template <typename KVT> constexpr int kPpThreads = 128 * kPpTiles + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
 constexpr float kPpLazy = 8.f;
 constexpr uint32_t kPpSpin = 1u << 24;
 
@@ -84,8 +85,24 @@ struct PromptSmem {
 };
 enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_O = 13, PB_COUNT = 15 };
 
-template <int HD>
-__global__ void __launch_bounds__(kPpThreads, 1)
+// 4-bit pages: eight codes (dims 0 .. 7) -> four bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code * scale / 256. Exponent and mantissa of
+// a code are put at the low end of a bf16's exponent, which makes it code * 2^-126 exactly (0.5 as a subnormal), and multiplied by `s`, the
+// block's scale * 2^118 twice. In that order a pair takes two shifts, two logic instructions and a product. (The conversion instruction
+// runs at a quarter of the rate of these and gives halves.)
+__device__ __forceinline__ uint4 widen_codes(uint32_t w, uint32_t s) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t sign = i < 3 ? w << (12 - 4 * i) : w, rest = i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6);
+        const uint32_t raw = (sign & 0x80008000u) | (rest & 0x01c001c0u);
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(raw), "r"(s));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+constexpr float kPpCodeScale = 256.f;            // what those values lack
+
+template <typename KVT, int HD>
+__global__ void __launch_bounds__(kPpThreads<KVT>, 1)
     attn_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnPagedParams p) {
     using L = PromptSmem<HD>;
     extern __shared__ unsigned char smem_raw[];
@@ -95,7 +112,8 @@ __global__ void __launch_bounds__(kPpThreads, 1)
     __shared__ uint32_t tmem_base;
     __shared__ int found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kLoader = 4 * kPpTiles, kIssuer = kLoader + 1;
+    constexpr bool Q4 = sizeof(KVT) == 1;
+    constexpr int kLoader = 4 * kPpTiles, kIssuer = kLoader + kPpLoaders<KVT>;
 
     if (warp == kLoader) {
         // which sequence's rows these are: those of sequences with more than kSplitRows, 256 at a time, later rows (which see more) first
@@ -126,7 +144,10 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         if (lane == 0) {
             found[0] = at;
             found[1] = want;
-            for (int i = 0; i < PB_COUNT; ++i) mbar_init(bar(i), i == PB_Q ? 128 * kPpTiles : i == PB_P || i == PB_P + 1 ? 128 : 1);
+            for (int i = 0; i < PB_COUNT; ++i) {
+                const bool filled = i == PB_KFULL || i == PB_KFULL + 1 || i == PB_VFULL || i == PB_VFULL + 1;
+                mbar_init(bar(i), i == PB_Q ? 128 * kPpTiles : i == PB_P || i == PB_P + 1 || (Q4 && filled) ? 128 : 1);
+            }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     }
@@ -152,7 +173,61 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         return false;
     };
 
-    if (warp == kLoader) {
+    if (Q4 && warp >= kLoader && warp < kIssuer) {
+        // a thread per position: its row of K, then of V, while the next step's codes are on their way
+        const int i = tid - 32 * kLoader;
+        constexpr int CW = HD / 8, SW = HD / 64;             // words of codes, of scales
+        uint32_t kc[CW], ks[SW], vc[CW], vs[SW];
+        auto load = [&](int j, bool is_k, uint32_t (&c)[CW], uint32_t (&sc)[SW]) {
+            const int v = j * kPpPages + i / kKvBlock, pg = v < span.count ? span.page(v) : 0, key = pg * kKvBlock + i % kKvBlock;
+            const bool use = v < span.count && key <= high && !(p.window > 0 && key <= low - p.window && key >= p.sinks);
+#pragma unroll
+            for (int e = 0; e < CW; ++e) c[e] = 0;
+#pragma unroll
+            for (int e = 0; e < SW; ++e) sc[e] = 0;
+            if (!use) return;
+            const size_t row = ((size_t)paged_page(p.c, p.r.err, b, pg, 0) * p.c.kv_heads + kvh) * kKvBlock + i % kKvBlock;
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(is_k ? p.c.kpool : p.c.vpool) + row * (HD / 2));
+            const uint32_t* ssrc = reinterpret_cast<const uint32_t*>((is_k ? p.c.kscale : p.c.vscale) + row * (HD / 16));
+#pragma unroll
+            for (int e = 0; e < CW / 4; ++e) {
+                const uint4 x = __ldg(src + e);
+                c[4 * e] = x.x; c[4 * e + 1] = x.y; c[4 * e + 2] = x.z; c[4 * e + 3] = x.w;
+            }
+#pragma unroll
+            for (int e = 0; e < SW; ++e) sc[e] = __ldg(ssrc + e);
+        };
+        auto store = [&](uint32_t at, const uint32_t (&c)[CW], const uint32_t (&sc)[SW]) {
+#pragma unroll
+            for (int e = 0; e < CW; e += 4) {                // two scales at a time
+                const uint32_t two = e4m3x2_to_f16(sc[e / 8] >> (e % 8 * 4));
+                const float a = f16_lo(two) * 3.3230699894622897e35f, d = f16_hi(two) * 3.3230699894622897e35f;      // 2^118
+                const uint32_t s0 = f32x2_to_bf16(a, a), s1 = f32x2_to_bf16(d, d);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int ch = e + u;
+                    *reinterpret_cast<uint4*>(sm + at + ch / 8 * L::kHalf + i * 128 + ((ch % 8) ^ (i & 7)) * 16) = widen_codes(c[ch], u < 2 ? s0 : s1);
+                }
+            }
+            fence_async_smem();
+        };
+        if (steps > 0) {
+            load(0, true, kc, ks);
+            load(0, false, vc, vs);
+        }
+        for (int j = 0; j < steps; ++j) {
+            const int st = j & 1;
+            const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+            if (!wait(PB_KEMPTY + st, ph ^ 1u)) break;
+            store(L::k + st * L::kKV, kc, ks);
+            mbar_arrive(bar(PB_KFULL + st));
+            if (j + 1 < steps) load(j + 1, true, kc, ks);
+            if (!wait(PB_VEMPTY + st, ph ^ 1u)) break;
+            store(L::v + st * L::kKV, vc, vs);
+            mbar_arrive(bar(PB_VFULL + st));
+            if (j + 1 < steps) load(j + 1, false, vc, vs);
+        }
+    } else if (!Q4 && warp == kLoader) {
         bool good = true;
         for (int j = 0; j < steps && good; ++j) {
             const int st = j & 1;
@@ -245,7 +320,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         const int pos = in ? pos0 + rr / p.group : high;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // the warp's 32 lanes of tensor memory
         // the row's queries, K-major with the swizzle that the MMA expects; a negative scale turns their sign
-        const float scale = p.scale * p.c.k_scale * 1.4426950408889634f;
+        const float scale = p.scale * p.c.k_scale * (Q4 ? kPpCodeScale : 1.f) * 1.4426950408889634f;
         {
             const bf16_t* q = static_cast<const bf16_t*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD;
             const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
@@ -264,6 +339,8 @@ __global__ void __launch_bounds__(kPpThreads, 1)
                         x = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     x.x ^= turn; x.y ^= turn; x.z ^= turn; x.w ^= turn;
+                    if (Q4)                                      // the order of dims in K
+                        x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
                 }
                 *reinterpret_cast<uint4*>(sm + L::q + t * L::kQ + c / 8 * L::kHalf + r * 128 + ((c % 8) ^ (r & 7)) * 16) = x;
             }
@@ -353,7 +430,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
                 tc_fence_after();
             }
             if (good) {
-                const float inv = pos < 0 ? 0.f : p.c.v_scale / l;
+                const float inv = pos < 0 ? 0.f : p.c.v_scale * (Q4 ? kPpCodeScale : 1.f) / l;
                 bool odd = false;
                 bf16_t* out = static_cast<bf16_t*>(p.out) + (size_t)row * p.out_stride + (size_t)h * HD;
                 const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
@@ -368,7 +445,8 @@ __global__ void __launch_bounds__(kPpThreads, 1)
                     float y[32];
 #pragma unroll
                     for (int u = 0; u < 32; ++u) {
-                        y[u] = pos < 0 ? 0.f : __uint_as_float(o[u]) * inv;
+                        const int from = !Q4 ? u : u / 8 * 8 + (u % 8 < 4 ? u % 8 * 2 : u % 8 * 2 - 7);      // the order of dims in V
+                        y[u] = pos < 0 ? 0.f : __uint_as_float(o[from]) * inv;
                         odd |= !(fabsf(y[u]) <= 3.4e38f);
                     }
                     if (p.gate && in) {
@@ -390,7 +468,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
                 }
                 for (unsigned again = __ballot_sync(0xffffffffu, odd && in); again; again &= again - 1) {
                     const int src = __ffs(again) - 1;
-                    careful_row<bf16_t, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
+                    careful_row<KVT, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
                 }
             }
         }
@@ -404,25 +482,29 @@ __global__ void __launch_bounds__(kPpThreads, 1)
     }
 }
 
-template <int HD>
+template <typename KVT, int HD>
 cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st) {
     alignas(64) CUtensorMap tk, tv;
+    std::memset(&tk, 0, sizeof tk);
+    std::memset(&tv, 0, sizeof tv);
     const uint64_t rows = (uint64_t)p.c.num_pages * p.c.kv_heads * kKvBlock;
-    if (make_bf16_map(enc, &tk, p.c.kpool, rows, HD, kKvBlock) || make_bf16_map(enc, &tv, p.c.vpool, rows, HD, kKvBlock)) return cudaErrorInvalidValue;
+    if (sizeof(KVT) == 2 && (make_bf16_map(enc, &tk, p.c.kpool, rows, HD, kKvBlock) || make_bf16_map(enc, &tv, p.c.vpool, rows, HD, kKvBlock)))
+        return cudaErrorInvalidValue;
     const size_t smem = PromptSmem<HD>::total + 1024;
-    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<KVT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles) + p.r.batch;
-    attn_prompt_kernel<HD><<<dim3((unsigned)tiles, p.c.kv_heads), kPpThreads, smem, st>>>(tk, tv, p);
+    attn_prompt_kernel<KVT, HD><<<dim3((unsigned)tiles, p.c.kv_heads), kPpThreads<KVT>, smem, st>>>(tk, tv, p);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t attn_prompt_launch(const AttnPagedParams& p, int head_dim, cudaStream_t st) {
+cudaError_t attn_prompt_launch(const AttnPagedParams& p, int dtype, int head_dim, cudaStream_t st) {
     static const EncodeTiledFn enc = get_encode_tiled();
     if (!enc) return cudaErrorNotSupported;
-    return head_dim == 64 ? launch<64>(enc, p, st) : launch<128>(enc, p, st);
+    if (dtype == MLB_DT_FP4_E2M1) return head_dim == 64 ? launch<fp4_t, 64>(enc, p, st) : launch<fp4_t, 128>(enc, p, st);
+    return head_dim == 64 ? launch<bf16_t, 64>(enc, p, st) : launch<bf16_t, 128>(enc, p, st);
 }
 
 }  // namespace mlb
