@@ -9,6 +9,7 @@
 // Positions that no row of the CTA sees (behind the last one, between the first positions and the window) are zeros in V: 0 times what
 // may lie there could be no number. A row whose result is not finite is done again from the formula (careful_row).
 #include <cstring>
+#include <type_traits>
 
 #include "paged_prompt.h"
 #include "paged_row.cuh"
@@ -55,6 +56,36 @@ __device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]), "r"(addr)
+                 : "memory");
+}
+// Largest of three; a NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// 2^x of two numbers, x <= 128, without the exponential's unit: x = n + r with n the nearest whole number, 2^r by the cubic 1 + r (a + r (b + r c))
+// whose largest relative error over -1/2 .. 1/2 is smallest (fitted by reweighted least squares: 1.0e-4, a twentieth of the half step of bf16
+// that the weight is rounded by next), n added to the exponent. Below 2^-126: about that.
+__device__ __forceinline__ f32x2 ex2_poly(f32x2 x) {
+    float a, d;
+    unpack2(x, a, d);
+    x = pack2(fmaxf(a, -126.f), fmaxf(d, -126.f));
+    const float big = 12582912.f;                // 1.5 * 2^23: whole numbers are its low bits
+    const f32x2 n = add2(x, pack2(big, big)), r = fma2(add2(n, pack2(-big, -big)), pack2(-1.f, -1.f), x);
+    f32x2 y = fma2(pack2(0.05500893f, 0.05500893f), r, pack2(0.24221100f, 0.24221100f));
+    y = fma2(y, r, pack2(0.69328290f, 0.69328290f));
+    y = fma2(y, r, pack2(1.f, 1.f));
+    float n0, n1;
+    unpack2(n, n0, n1);
+    unpack2(y, a, d);
+    return pack2u(__float_as_uint(a) + (__float_as_uint(n0) << 23), __float_as_uint(d) + (__float_as_uint(n1) << 23));
+}
+
 // B operand whose N runs along the 128-byte rows (V: a row is a position, the dims are N): 64 dims a row, 128-byte swizzle, groups of
 // eight positions 1024 bytes apart, the next 64 dims `next` bytes on.
 __device__ __forceinline__ uint64_t umma_desc_rows_are_k(uint32_t smem_addr, uint32_t next) {
@@ -83,7 +114,7 @@ struct PromptSmem {
     static constexpr uint32_t kQ = 128 * HD * 2, kKV = kPpKeys * HD * 2, kHalf = 128 * 128;      // bytes of a tile; of 64 dims of one
     static constexpr uint32_t q = 0, k = kPpTiles * kQ, v = k + 2 * kKV, bars = v + 2 * kKV, total = bars + 256;
 };
-enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_O = 13, PB_COUNT = 15 };
+enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_COUNT = 17 };
 
 // 4-bit pages: eight codes (dims 0 .. 7) -> four bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code * scale / 256. Exponent and mantissa of
 // a code are put at the low end of a bf16's exponent, which makes it code * 2^-126 exactly (0.5 as a subnormal), and multiplied by `s`, the
@@ -146,7 +177,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
             found[1] = want;
             for (int i = 0; i < PB_COUNT; ++i) {
                 const bool filled = i == PB_KFULL || i == PB_KFULL + 1 || i == PB_VFULL || i == PB_VFULL + 1;
-                mbar_init(bar(i), i == PB_Q ? 128 * kPpTiles : i == PB_P || i == PB_P + 1 || (Q4 && filled) ? 128 : 1);
+                mbar_init(bar(i), i == PB_Q ? 128 * kPpTiles : (i >= PB_P && i < PB_O) || (Q4 && filled) ? 128 : 1);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -295,9 +326,16 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                     if (!good) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < kPpKeys / 16; ++ks)
+                    for (int ks = 0; ks < kPpKeys / 16; ++ks) {
+                        if (ks == kPpKeys / 32) {
+                            good = wait(PB_P2 + t, (uint32_t)j & 1u);
+                            if (!good) break;
+                            tc_fence_after();
+                        }
                         umma_bf16_ta(tmem + (2 + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + (j & 1) * L::kKV + ks * 2048, L::kHalf), io,
                                      j > 0 || ks > 0);
+                    }
+                    if (!good) break;
                     if (t == tiles - 1) umma_commit(bar(PB_VEMPTY + (j & 1)));
                     if (j + 1 < steps) {
                         if (t == 0) {
@@ -356,37 +394,43 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                 good = __all_sync(0xffffffffu, wait(PB_S + t, (uint32_t)j & 1u));
                 if (!good) break;
                 tc_fence_after();
-                uint32_t x[4][32];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) tmem_ld32(tmem + lanes + t * 128 + e * 32, x[e]);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 4; ++e) tmem_loaded(x[e]);
                 // positions that some row of the warp does not see
                 bool edge = (j + 1) * kPpPages > span.count;
                 if (!edge) {
                     const int ka = span.page(j * kPpPages) * kKvBlock, kb = span.page(j * kPpPages + kPpPages - 1) * kKvBlock + kKvBlock - 1;
                     edge = kb > wlow || (p.window > 0 && ka <= whigh - p.window && !(kb < p.sinks));
                 }
-                if (edge) {
+                // 32 positions from 32 g on: those that the row does not see to -inf
+                auto hide = [&](uint32_t (&x)[32], int g) {
 #pragma unroll
-                    for (int g = 0; g < kPpPages; ++g) {
-                        const int v = j * kPpPages + g, k0 = v < span.count ? span.page(v) * kKvBlock : 0x40000000;
+                    for (int u = 0; u < 2; ++u) {
+                        const int v = j * kPpPages + 2 * g + u, k0 = v < span.count ? span.page(v) * kKvBlock : 0x40000000;
                         const int hi = pos - k0, lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) - k0, sk = p.sinks - k0;
 #pragma unroll
-                        for (int e = 0; e < kKvBlock; ++e) {
-                            const int at = g * kKvBlock + e;
-                            if (!(e <= hi && (e >= lo || e < sk))) x[at / 32][at % 32] = 0xff800000u;      // -inf
-                        }
+                        for (int e = 0; e < kKvBlock; ++e)
+                            if (!(e <= hi && (e >= lo || e < sk))) x[u * kKvBlock + e] = 0xff800000u;
                     }
+                };
+                const uint32_t sc = tmem + lanes + t * 128;
+                // The scores are read twice, for the maximum and for the weights: held in between, 128 registers of a thread would be theirs.
+                float mx;
+                {
+                    uint32_t x[2][32];
+                    float top[2] = {-INFINITY, -INFINITY};
+                    tmem_ld32(sc, x[0]);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        tmem_ld_wait();
+                        tmem_loaded(x[g & 1]);
+                        if (g < 3) tmem_ld32(sc + 32 * (g + 1), x[(g + 1) & 1]);
+                        if (edge) hide(x[g & 1], g);
+#pragma unroll
+                        for (int u = 0; u < 32; u += 2)
+                            top[u / 2 & 1] = max3_nan(top[u / 2 & 1], __uint_as_float(x[g & 1][u]), __uint_as_float(x[g & 1][u + 1]));
+                    }
+                    mx = max3_nan(top[0], top[1], -INFINITY) * c;
                 }
-                float top[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top[e] = __uint_as_float(x[0][e]);
-#pragma unroll
-                for (int at = 8; at < kPpKeys; ++at) top[at % 8] = fmaxf(top[at % 8], __uint_as_float(x[at / 32][at % 32]));
-                const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7]))) * c;
-                const bool moved = mx > m + kPpLazy;
+                const bool moved = !(mx <= m + kPpLazy);      // (a score that is no number makes the maximum, and so the row, none)
                 if (__any_sync(0xffffffffu, moved)) {
                     const float f = moved ? ex2(m - mx) : 1.f;
                     if (moved) m = mx;
@@ -405,24 +449,53 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const f32x2 cc = pack2(c, c), rr2 = pack2(-ref, -ref);
+                f32x2 sum[2] = {0ull, 0ull};
+                // weights of 32 positions, one pair of four by polynomial: the exponential's unit takes 16 a cycle and would be the bound
+                auto weigh = [&](auto by_unit, const uint32_t (&x)[32], uint32_t (&w)[16]) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int u = 0; u < 32; ++u) {
-                        const int at = half * 64 + 2 * u;
-                        const float a = ex2(fmaf(__uint_as_float(x[at / 32][at % 32]), c, -ref)), d = ex2(fmaf(__uint_as_float(x[at / 32][at % 32 + 1]), c, -ref));
-                        sum[u % 2 * 2] += a;
-                        sum[u % 2 * 2 + 1] += d;
+                    for (int u = 0; u < 16; ++u) {
+                        f32x2 y = fma2(pack2u(x[2 * u], x[2 * u + 1]), cc, rr2);
+                        float a, d;
+                        if (!decltype(by_unit)::value && u % 4 == 3) {
+                            y = ex2_poly(y);
+                            unpack2(y, a, d);
+                        } else {
+                            unpack2(y, a, d);
+                            a = ex2(a);
+                            d = ex2(d);
+                            y = pack2(a, d);
+                        }
+                        sum[u & 1] = add2(sum[u & 1], y);
                         w[u] = f32x2_to_bf16(a, d);
                     }
-                    tmem_st32(tmem + lanes + t * 128 + half * 32, w);
+                };
+                {
+                    uint32_t x[2][32], w[16];
+                    tmem_ld32(sc, x[0]);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        tmem_ld_wait();
+                        tmem_loaded(x[g & 1]);
+                        if (g < 3) tmem_ld32(sc + 32 * (g + 1), x[(g + 1) & 1]);
+                        if (edge) {
+                            hide(x[g & 1], g);
+                            weigh(std::true_type(), x[g & 1], w);      // exactly 0 where hidden
+                        } else {
+                            weigh(std::false_type(), x[g & 1], w);
+                        }
+                        tmem_st16(sc + 16 * g, w);               // over scores that have been read
+                        if (g & 1) {                             // half of the positions: their products can begin
+                            tmem_st_wait();
+                            tc_fence_before();
+                            mbar_arrive(bar((g == 1 ? PB_P : PB_P2) + t));
+                        }
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(bar(PB_P + t));
+                float sa, sb, sd, se;
+                unpack2(sum[0], sa, sb);
+                unpack2(sum[1], sd, se);
+                l += (sa + sb) + (sd + se);
             }
             // results
             if (steps > 0 && good) {
