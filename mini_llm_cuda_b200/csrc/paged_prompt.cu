@@ -19,11 +19,13 @@ namespace mlb {
 
 namespace {
 
-constexpr int kPpTiles = 2;
+// Tiles of 128 rows of a CTA. One, and two CTAs on an SM, where TMA brings K and V: the CTAs alternate on the tensor core as the tiles of one would, and
+// one's start and end lie under the other's steps. Two where warps widen 4-bit pages, which serves both.
+template <typename KVT> constexpr int kPpTiles = sizeof(KVT) == 1 ? 2 : 1;
 constexpr int kPpKeys = 128;                     // positions of a step
 constexpr int kPpPages = kPpKeys / kKvBlock;
 template <typename KVT> constexpr int kPpLoaders = sizeof(KVT) == 1 ? 4 : 1;                             // warps that bring K and V
-template <typename KVT> constexpr int kPpThreads = 128 * kPpTiles + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
+template <typename KVT> constexpr int kPpThreads = 128 * kPpTiles<KVT> + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
 constexpr float kPpLazy = 8.f;
 constexpr uint32_t kPpSpin = 1u << 24;
 
@@ -109,10 +111,11 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, u
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <int HD>
+template <int HD, int TILES>
 struct PromptSmem {
+    static constexpr int stages = TILES;         // of K and V: with one, the other CTA of the SM fills the wait
     static constexpr uint32_t kQ = 128 * HD * 2, kKV = kPpKeys * HD * 2, kHalf = 128 * 128;      // bytes of a tile; of 64 dims of one
-    static constexpr uint32_t q = 0, k = kPpTiles * kQ, v = k + 2 * kKV, bars = v + 2 * kKV, total = bars + 256;
+    static constexpr uint32_t q = 0, k = TILES * kQ, v = k + stages * kKV, bars = v + stages * kKV, total = bars + 256;
 };
 enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_COUNT = 17 };
 
@@ -133,29 +136,37 @@ __device__ __forceinline__ uint4 widen_codes(uint32_t w, uint32_t s) {
 constexpr float kPpCodeScale = 256.f;            // what those values lack
 
 template <typename KVT, int HD>
-__global__ void __launch_bounds__(kPpThreads<KVT>, 1)
+__global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     attn_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnPagedParams p) {
-    using L = PromptSmem<HD>;
+    constexpr int TILES = kPpTiles<KVT>;
+    using L = PromptSmem<HD, TILES>;
+    constexpr int NST = L::stages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sm0 = smem_u32(sm), bar0 = sm0 + L::bars;
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     __shared__ uint32_t tmem_base;
-    __shared__ int found[2];
+    __shared__ int found[5];                     // sequence, tile in it, the sequence's first row, rows, positions
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr bool Q4 = sizeof(KVT) == 1;
-    constexpr int kLoader = 4 * kPpTiles, kIssuer = kLoader + kPpLoaders<KVT>;
+    constexpr int kLoader = 4 * TILES, kIssuer = kLoader + kPpLoaders<KVT>;
 
+    if (warp == kIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256u * TILES) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tc_fence_before();
+    }
     if (warp == kLoader) {
-        // which sequence's rows these are: those of sequences with more than kSplitRows, 256 at a time, later rows (which see more) first
+        // which sequence's rows these are: those of sequences with more than kSplitRows, 128 TILES at a time, later rows (which see more) first
         int want = (int)(gridDim.x - 1 - blockIdx.x), at = -1;
         for (int b0 = 0; b0 < p.r.batch && at < 0; b0 += 32) {
             const int b = b0 + lane;
             int n = 0;
+            PagedSeq s = {0, 0, 0};
             if (b < p.r.batch) {
-                const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0 && blockIdx.y == 0);
+                s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0 && blockIdx.y == 0);
                 const long long rows = (long long)s.n * p.group;
-                n = rows > kSplitRows ? (int)((rows + 128 * kPpTiles - 1) / (128 * kPpTiles)) : 0;
+                n = rows > kSplitRows ? (int)((rows + 128 * TILES - 1) / (128 * TILES)) : 0;
             }
             int x = n;
 #pragma unroll
@@ -168,6 +179,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                 const int src = __ffs(has) - 1;
                 at = b0 + src;
                 want -= __shfl_sync(0xffffffffu, x - n, src);
+                if (lane == src) { found[2] = s.r0; found[3] = s.n; found[4] = s.len; }
             } else {
                 want -= __shfl_sync(0xffffffffu, x, 31);
             }
@@ -177,24 +189,22 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
             found[1] = want;
             for (int i = 0; i < PB_COUNT; ++i) {
                 const bool filled = i == PB_KFULL || i == PB_KFULL + 1 || i == PB_VFULL || i == PB_VFULL + 1;
-                mbar_init(bar(i), i == PB_Q ? 128 * kPpTiles : (i >= PB_P && i < PB_O) || (Q4 && filled) ? 128 : 1);
+                mbar_init(bar(i), i == PB_Q ? 128 * TILES : (i >= PB_P && i < PB_O) || (Q4 && filled) ? 128 : 1);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     }
     __syncthreads();
-    if (found[0] < 0) return;                    // (uniform)
-    if (warp == kIssuer) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-        tc_fence_before();
-    }
-    __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base;             // S0 | S1 | O0 | O1, 128 columns each
-    const int b = found[0], kvh = blockIdx.y, first = found[1] * 128 * kPpTiles;
-    const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, false);
-    const int count = min(128 * kPpTiles, s.n * p.group - first), tiles = count > 128 ? 2 : 1;
+    const uint32_t tmem = tmem_base;             // S of each tile, then O of each, 128 columns apart
+    auto release = [&]() { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * TILES)); };
+    if (found[0] < 0) {                          // (uniform)
+        if (warp == kIssuer) release();
+        return;
+    }
+    const int b = found[0], kvh = blockIdx.y, first = found[1] * 128 * TILES;
+    const PagedSeq s = {found[2], found[3], found[4]};
+    const int count = min(128 * TILES, s.n * p.group - first), tiles = TILES == 2 && count > 128 ? 2 : 1;
     const int pos0 = s.len - s.n, low = pos0 + first / p.group, high = pos0 + (first + count - 1) / p.group;
     const PagedSpan span = paged_span(p, low, high);
     const int steps = (span.count + kPpPages - 1) / kPpPages;
@@ -247,8 +257,8 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
             load(0, false, vc, vs);
         }
         for (int j = 0; j < steps; ++j) {
-            const int st = j & 1;
-            const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+            const int st = j % NST;
+            const uint32_t ph = (uint32_t)(j / NST) & 1u;
             if (!wait(PB_KEMPTY + st, ph ^ 1u)) break;
             store(L::k + st * L::kKV, kc, ks);
             mbar_arrive(bar(PB_KFULL + st));
@@ -261,8 +271,8 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
     } else if (!Q4 && warp == kLoader) {
         bool good = true;
         for (int j = 0; j < steps && good; ++j) {
-            const int st = j & 1;
-            const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+            const int st = j % NST;
+            const uint32_t ph = (uint32_t)(j / NST) & 1u;
             const int v = j * kPpPages + (lane & 7), pg = v < span.count ? span.page(v) : 0;
             const bool held = lane < kPpPages && v < span.count;
             const int row0 = held ? (int)(((long long)paged_page(p.c, p.r.err, b, pg, 0) * p.c.kv_heads + kvh) * kKvBlock) : 0;
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const uint32_t off = (uint32_t)(ks / 4) * L::kHalf + (uint32_t)(ks % 4) * 32;
-                    umma_bf16(tmem + t * 128, umma_desc_sw128(sm0 + L::q + t * L::kQ + off), umma_desc_sw128(sm0 + L::k + (j & 1) * L::kKV + off), is, ks > 0);
+                    umma_bf16(tmem + t * 128, umma_desc_sw128(sm0 + L::q + t * L::kQ + off), umma_desc_sw128(sm0 + L::k + j % NST * L::kKV + off), is, ks > 0);
                 }
                 umma_commit(bar(PB_S + t));
             };
@@ -320,9 +330,9 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                 umma_commit(bar(PB_KEMPTY));
             }
             for (int j = 0; j < steps && good; ++j) {
-                const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+                const uint32_t ph = (uint32_t)(j / NST) & 1u;
                 for (int t = 0; t < tiles && good; ++t) {
-                    good = wait(PB_P + t, (uint32_t)j & 1u) && (t > 0 || wait(PB_VFULL + (j & 1), ph));
+                    good = wait(PB_P + t, (uint32_t)j & 1u) && (t > 0 || wait(PB_VFULL + j % NST, ph));
                     if (!good) break;
                     tc_fence_after();
 #pragma unroll
@@ -332,19 +342,19 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                             if (!good) break;
                             tc_fence_after();
                         }
-                        umma_bf16_ta(tmem + (2 + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + (j & 1) * L::kKV + ks * 2048, L::kHalf), io,
+                        umma_bf16_ta(tmem + (TILES + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
                                      j > 0 || ks > 0);
                     }
                     if (!good) break;
-                    if (t == tiles - 1) umma_commit(bar(PB_VEMPTY + (j & 1)));
+                    if (t == tiles - 1) umma_commit(bar(PB_VEMPTY + j % NST));
                     if (j + 1 < steps) {
                         if (t == 0) {
-                            good = wait(PB_KFULL + ((j + 1) & 1), (((uint32_t)j + 1) >> 1) & 1u);
+                            good = wait(PB_KFULL + (j + 1) % NST, (uint32_t)((j + 1) / NST) & 1u);
                             if (!good) break;
                             tc_fence_after();
                         }
                         scores(t, j + 1);
-                        if (t == tiles - 1) umma_commit(bar(PB_KEMPTY + ((j + 1) & 1)));
+                        if (t == tiles - 1) umma_commit(bar(PB_KEMPTY + (j + 1) % NST));
                     } else {
                         umma_commit(bar(PB_O + t));
                     }
@@ -439,12 +449,12 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
 #pragma unroll 1
                         for (int e = 0; e < HD / 32; ++e) {
                             uint32_t o[32];
-                            tmem_ld32(tmem + lanes + (2 + t) * 128 + e * 32, o);
+                            tmem_ld32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
                             tmem_ld_wait();
                             tmem_loaded(o);
 #pragma unroll
                             for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
-                            tmem_st32(tmem + lanes + (2 + t) * 128 + e * 32, o);
+                            tmem_st32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
                         }
                     }
                 }
@@ -511,7 +521,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
                 for (int e = 0; e < HD / 32; ++e) {
                     uint32_t o[32];
                     if (steps > 0) {
-                        tmem_ld32(tmem + lanes + (2 + t) * 128 + e * 32, o);
+                        tmem_ld32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
                         tmem_ld_wait();
                         tmem_loaded(o);
                     }
@@ -551,7 +561,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 1)
     __syncthreads();
     if (warp == kIssuer) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+        release();
     }
 }
 
@@ -563,10 +573,10 @@ cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st)
     const uint64_t rows = (uint64_t)p.c.num_pages * p.c.kv_heads * kKvBlock;
     if (sizeof(KVT) == 2 && (make_bf16_map(enc, &tk, p.c.kpool, rows, HD, kKvBlock) || make_bf16_map(enc, &tv, p.c.vpool, rows, HD, kKvBlock)))
         return cudaErrorInvalidValue;
-    const size_t smem = PromptSmem<HD>::total + 1024;
+    const size_t smem = PromptSmem<HD, kPpTiles<KVT>>::total + 1024;
     cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<KVT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles) + p.r.batch;
+    const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles<KVT>) + p.r.batch;
     attn_prompt_kernel<KVT, HD><<<dim3((unsigned)tiles, p.c.kv_heads), kPpThreads<KVT>, smem, st>>>(tk, tv, p);
     return cudaGetLastError();
 }
