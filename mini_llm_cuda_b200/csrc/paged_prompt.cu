@@ -3,7 +3,7 @@
 // A CTA takes 256 consecutive (token, query head) rows of one K/V head, as two tiles of 128, through the pages that any of them sees, 128
 // positions at a time:  S = Q K^T, P = exp2(S - m), O += P V. S (fp32) and O lie in tensor memory, P as bf16 over the columns of its S, so
 // that it is the MMA's A operand from there. One warp brings K and V (TMA, a page at a time: 16 rows of 128-byte swizzled halves), one
-// thread issues the MMAs, and four warps per tile take a row per thread: maximum, exponentials, sum, without any exchange between threads.
+// issues the MMAs, and four warps per tile take a row per thread: maximum, exponentials, sum, without any exchange between threads.
 // The two tiles alternate on the tensor core: while one's products run, the other's exponentials are taken.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the reference of its weights was set.
 // Positions that no row of the CTA sees (behind the last one, between the first positions and the window) are zeros in V: 0 times what
@@ -99,14 +99,38 @@ __device__ __forceinline__ uint64_t umma_desc_rows_are_k(uint32_t smem_addr, uin
     d |= (uint64_t)2 << 61;
     return d;
 }
-__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// MMAs and commits are issued by a whole warp that elects a lane for each. Issued under `if (lane == 0)` an MMA took 100 to 215 cycles,
+// whatever its size, since its operands have to be brought into uniform registers lane by lane there; this way 64, the tensor core's own
+// for 128 x 128 x 16.
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, one;\n"
         "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "elect.sync _|one, 0xffffffff;\n"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, one;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "elect.sync _|one, 0xffffffff;\n"
+        "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
         "}\n" ::"r"(tmem_d),
         "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint32_t mbar) {
+    asm volatile(
+        "{\n"
+        ".reg .pred one;\n"
+        "elect.sync _|one, 0xffffffff;\n"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        "}\n" ::"r"(mbar)
         : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -196,7 +220,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base;             // S of each tile, then O of each, 128 columns apart
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);             // S of each tile, then O of each, 128 columns apart
     auto release = [&]() { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * TILES)); };
     if (found[0] < 0) {                          // (uniform)
         if (warp == kIssuer) release();
@@ -313,50 +337,51 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             }
         }
     } else if (warp == kIssuer) {
-        if (lane == 0 && steps > 0) {
+        if (steps > 0) {
             const uint32_t is = umma_idesc_bf16(128, kPpKeys), io = umma_idesc_bf16(128, HD) | (1u << 16);      // bit 16: N runs along B's rows
             auto scores = [&](int t, int j) {
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const uint32_t off = (uint32_t)(ks / 4) * L::kHalf + (uint32_t)(ks % 4) * 32;
-                    umma_bf16(tmem + t * 128, umma_desc_sw128(sm0 + L::q + t * L::kQ + off), umma_desc_sw128(sm0 + L::k + j % NST * L::kKV + off), is, ks > 0);
+                    umma_ss(tmem + t * 128, umma_desc_sw128(sm0 + L::q + t * L::kQ + off), umma_desc_sw128(sm0 + L::k + j % NST * L::kKV + off), is, ks > 0);
                 }
-                umma_commit(bar(PB_S + t));
+                commit_elected(bar(PB_S + t));
             };
-            bool good = wait(PB_Q, 0) && wait(PB_KFULL, 0);
+            auto all_wait = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, wait(i, parity)) != 0; };
+            bool good = all_wait(PB_Q, 0) && all_wait(PB_KFULL, 0);
             tc_fence_after();
             if (good) {
                 for (int t = 0; t < tiles; ++t) scores(t, 0);
-                umma_commit(bar(PB_KEMPTY));
+                commit_elected(bar(PB_KEMPTY));
             }
             for (int j = 0; j < steps && good; ++j) {
                 const uint32_t ph = (uint32_t)(j / NST) & 1u;
                 for (int t = 0; t < tiles && good; ++t) {
-                    good = wait(PB_P + t, (uint32_t)j & 1u) && (t > 0 || wait(PB_VFULL + j % NST, ph));
+                    good = all_wait(PB_P + t, (uint32_t)j & 1u) && (t > 0 || all_wait(PB_VFULL + j % NST, ph));
                     if (!good) break;
                     tc_fence_after();
 #pragma unroll
                     for (int ks = 0; ks < kPpKeys / 16; ++ks) {
                         if (ks == kPpKeys / 32) {
-                            good = wait(PB_P2 + t, (uint32_t)j & 1u);
+                            good = all_wait(PB_P2 + t, (uint32_t)j & 1u);
                             if (!good) break;
                             tc_fence_after();
                         }
-                        umma_bf16_ta(tmem + (TILES + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
+                        umma_ts(tmem + (TILES + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
                                      j > 0 || ks > 0);
                     }
                     if (!good) break;
-                    if (t == tiles - 1) umma_commit(bar(PB_VEMPTY + j % NST));
+                    if (t == tiles - 1) commit_elected(bar(PB_VEMPTY + j % NST));
                     if (j + 1 < steps) {
                         if (t == 0) {
-                            good = wait(PB_KFULL + (j + 1) % NST, (uint32_t)((j + 1) / NST) & 1u);
+                            good = all_wait(PB_KFULL + (j + 1) % NST, (uint32_t)((j + 1) / NST) & 1u);
                             if (!good) break;
                             tc_fence_after();
                         }
                         scores(t, j + 1);
-                        if (t == tiles - 1) umma_commit(bar(PB_KEMPTY + (j + 1) % NST));
+                        if (t == tiles - 1) commit_elected(bar(PB_KEMPTY + (j + 1) % NST));
                     } else {
-                        umma_commit(bar(PB_O + t));
+                        commit_elected(bar(PB_O + t));
                     }
                 }
             }
