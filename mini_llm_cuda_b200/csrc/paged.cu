@@ -95,9 +95,12 @@ PagedRows rows_of(const mlb_ops* o, const mlb_new_rows* r) {
 }
 
 // ---- append and read ---------------------------------------------------------------------------------------------
-// A thread takes eight dims of one head of one row: 16 bytes of bf16 rows, 32 of fp32. K heads first, then V heads, then (append) the
-// query heads. Both kernels are bound by HBM, or by their launch.
-constexpr int kMoveThreads = 256;
+// A CTA takes up to kMoveRows rows. Its warps look up where these stand (sequence, position, page) first, a row each. Then a thread takes eight dims
+// (16 bytes of bf16 rows, 32 of fp32) of one head of all of the rows, so that what depends on the head alone is worked out once, and goes on to
+// another head where there are more than the CTA's threads hold. K heads first, then V heads, then (append) the query heads. Bound by HBM, or by the
+// launch. A thread per eight dims of the call, each of which looked up its own row, executed 300 instructions for them and was bound by
+// these: 125 us for 16001 rows of 32 + 2 x 8 heads of 128, bf16, into 4 bits, and 37 us to read K and V back; 76 and 23 this way, 4.7 and 3.7 TB/s.
+constexpr int kMoveThreads = 256, kMoveRows = 8;
 
 struct MoveParams {
     PagedCache c;
@@ -109,28 +112,45 @@ struct MoveParams {
     const float* rope; int rope_len;
     int heads;                                   // query heads, 0 without them
     int vec;                                     // all rows (and the table) start on 16 bytes
+    int cta_rows;                                // rows of a CTA
 };
 
+// Eight numbers as they lie in memory
 template <typename RT>
-__device__ __forceinline__ void load8(const RT* p, bool vec, float (&x)[8]) {
-    if (vec) {
-        if (sizeof(RT) == 2) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Raw8 {
+    uint4 w[sizeof(RT) / 2];
+    __device__ __forceinline__ void load(const RT* p, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(RT) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else if constexpr (sizeof(RT) == 2) {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = (uint32_t)__bfloat16_as_ushort(p[2 * i]) | (uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) << 16;
+            w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[i] = make_uint4(__float_as_uint(p[4 * i]), __float_as_uint(p[4 * i + 1]), __float_as_uint(p[4 * i + 2]), __float_as_uint(p[4 * i + 3]));
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        if constexpr (sizeof(RT) == 2) {
+            const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[2 * i] = __uint_as_float(u[i] << 16);
                 x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
             }
         } else {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = Elem<RT>::get(p, i);
+            for (int i = 0; i < 2; ++i) {
+                x[4 * i] = __uint_as_float(w[i].x); x[4 * i + 1] = __uint_as_float(w[i].y);
+                x[4 * i + 2] = __uint_as_float(w[i].z); x[4 * i + 3] = __uint_as_float(w[i].w);
+            }
+        }
     }
-}
+};
 template <typename RT>
 __device__ __forceinline__ void store8(RT* p, bool vec, const float (&x)[8]) {
     if (vec) {
@@ -166,122 +186,159 @@ __device__ __forceinline__ int find_seq(const int* row_start, int batch, int t) 
     return lo;
 }
 
-// Row t's sequence, of a CTA whose first row's is b0; false: the row belongs to none that can be used, or is padding
-__device__ __forceinline__ bool place(const PagedRows& r, int pt_stride, int b0, int t, int& b, int& pos) {
-    b = b0;
-    if (r.row_start)
-        while (b + 1 < r.batch && r.row_start[b + 1] <= t) ++b;
-    const PagedSeq s = paged_seq(r, pt_stride, b, true);
-    if (t < s.r0 || t >= s.r0 + s.n) return false;
-    pos = s.len - s.n + (t - s.r0);
-    return pos >= 0;
-}
-
 template <typename KVT, typename RT, int HD, bool READ>
-__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ MoveParams p) {
+__global__ void __launch_bounds__(kMoveThreads, 4) kv_move_kernel(const __grid_constant__ MoveParams p) {
     constexpr int PER = HD / 8;                  // threads of a head
-    __shared__ int sb;
-    const int units = (2 * p.c.kv_heads + (READ ? 0 : p.heads)) * PER;      // of a row
-    const int first = (int)blockIdx.x * kMoveThreads, i = first + (int)threadIdx.x;
+    constexpr bool Q4 = sizeof(KVT) == 1;
+    __shared__ int place[kMoveRows];             // position; negative: nothing to do
+    __shared__ long long pool_row[kMoveRows];    // row of the pools, of head 0; negative: none to write to
+    __shared__ float4 turns[READ ? 1 : kMoveRows][2][PER];        // the rows' (cos, sin): first four and last four of a thread's eight numbers
+    const int tid = threadIdx.x, first = (int)blockIdx.x * p.cta_rows, n = min(p.cta_rows, p.r.rows - first);
+    for (int i = tid / 32; i < n; i += (int)blockDim.x / 32) {
+        const int t = first + i, b = p.r.row_start ? find_seq(p.r.row_start, p.r.batch, t) : t;
+        if (tid % 32 == 0) {
+            int pos = -1, page = -1;
+            if (b < p.r.batch) {
+                const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, true);
+                if (t >= s.r0 && t < s.r0 + s.n) pos = s.len - s.n + (t - s.r0);
+            }
+            if (!READ && p.rope && pos >= p.rope_len) {
+                atomicExch(p.r.err, PG_ROPE);
+                pos = -1;
+            }
+            if (pos >= 0) page = paged_page(p.c, p.r.err, b, pos / kKvBlock, READ ? 0 : -1);
+            place[i] = pos;
+            pool_row[i] = page < 0 ? -1 : (long long)page * p.c.kv_heads * kKvBlock + pos % kKvBlock;
+        }
+    }
+    __syncthreads();
     const bool vec = p.vec != 0;
-    if (p.r.row_start) {
-        if (threadIdx.x < 32) {
-            const int b = find_seq(p.r.row_start, p.r.batch, first / units);
-            if (threadIdx.x == 0) sb = b;
+    if (!READ && p.rope) {
+        for (int i = tid; i < n * PER; i += (int)blockDim.x) {
+            const int r = i / PER, c = i % PER;
+            if (place[r] < 0) continue;
+            Raw8<float> w;
+            float x[8];
+            w.load(p.rope + (size_t)place[r] * HD + c * 8, vec);
+            w.get(x);
+            turns[r][0][c] = make_float4(x[0], x[1], x[2], x[3]);
+            turns[r][1][c] = make_float4(x[4], x[5], x[6], x[7]);
         }
         __syncthreads();
     }
-    const int t = i / units;
-    int b, pos = 0;
-    // (threads past the last row stay to the end: the shuffles below want whole warps)
-    const bool used = t < p.r.rows && (p.r.row_start || t < p.r.batch) && place(p.r, p.c.pt_stride, p.r.row_start ? sb : t, t, b, pos);
-    const int u = i - t * units, head = u / PER, e = u % PER * 8;
-    const bool is_k = head < p.c.kv_heads, is_v = !is_k && head < 2 * p.c.kv_heads;
-    const int h = is_k ? head : is_v ? head - p.c.kv_heads : head - 2 * p.c.kv_heads;
-    bool good = used;
-    if (!READ && p.rope && good && pos >= p.rope_len) {
-        atomicExch(p.r.err, PG_ROPE);
-        good = false;
-    }
-    size_t row = 0;                              // row of the pools
-    if (good && (is_k || is_v)) {
-        const int page = paged_page(p.c, p.r.err, b, pos / kKvBlock, READ ? 0 : -1);
-        good = page >= 0;
-        row = ((size_t)max(page, 0) * p.c.kv_heads + h) * kKvBlock + pos % kKvBlock;
-    }
-    float x[8];
-    if (READ) {
-        if (!good) return;
-        const void* pool = is_k ? p.c.kpool : p.c.vpool;
-        if constexpr (sizeof(KVT) == 1) {
-            const uint32_t codes = *reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(pool) + row * (HD / 2) + e / 2);
-            const float s = e4m3_to_f32((is_k ? p.c.kscale : p.c.vscale)[row * (HD / 16) + e / 16]), g = is_k ? p.c.k_scale : p.c.v_scale;
-            uint32_t w[4];
-            e2m1x8_to_f16(codes, w);
+    const int heads = 2 * p.c.kv_heads + (READ ? 0 : p.heads), e = tid % PER * 8;
+    for (int h0 = 0; h0 < heads; h0 += (int)blockDim.x / PER) {
+        const int head = h0 + tid / PER;
+        const bool in = head < heads, is_k = head < p.c.kv_heads, is_v = !is_k && head < 2 * p.c.kv_heads, pooled = is_k || is_v;
+        const int h = is_k ? head : is_v ? head - p.c.kv_heads : head - 2 * p.c.kv_heads;
+        // this thread's place in row `first` of the caller's tensor, and in row 0 of the head's in a page
+        const long long stride = is_k ? p.k_stride : is_v ? p.v_stride : p.q_stride;
+        const size_t at = first * stride + h * HD + e;
+        unsigned char* const pool = static_cast<unsigned char*>(is_k ? p.c.kpool : p.c.vpool) + (Q4 ? ((size_t)h * kKvBlock * HD + e) / 2 : ((size_t)h * kKvBlock * HD + e) * sizeof(KVT));
+        unsigned char* const scales = Q4 ? (is_k ? p.c.kscale : p.c.vscale) + ((size_t)h * kKvBlock * HD + e) / 16 : nullptr;
+        const float g = is_k ? p.c.k_scale : p.c.v_scale;
+        if constexpr (READ) {
+            RT* dst = static_cast<RT*>(is_k ? p.k_out : p.v_out) + at;
+            if (!in) break;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i, dst += stride) {
+                if (place[i] < 0) continue;
+                const size_t row = (size_t)pool_row[i];
+                float x[8];
+                if constexpr (Q4) {
+                    const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(pool + row * (HD / 2)));
+                    const float s = e4m3_to_f32(__ldg(scales + row * (HD / 16)));
+                    uint32_t w[4];
+                    e2m1x8_to_f16(codes, w);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[2 * j] = __fmul_rn(__fmul_rn(f16_lo(w[j]), s), g);
-                x[2 * j + 1] = __fmul_rn(__fmul_rn(f16_hi(w[j]), s), g);
+                    for (int j = 0; j < 4; ++j) {
+                        x[2 * j] = __fmul_rn(__fmul_rn(f16_lo(w[j]), s), g);
+                        x[2 * j + 1] = __fmul_rn(__fmul_rn(f16_hi(w[j]), s), g);
+                    }
+                } else {
+                    Raw8<KVT> raw;
+                    raw.load(reinterpret_cast<const KVT*>(pool) + row * HD, true);
+                    raw.get(x);
+                }
+                store8(dst, vec, x);
             }
         } else {
-            load8(static_cast<const KVT*>(pool) + row * HD + e, true, x);
-        }
-        if (is_k) store8(static_cast<RT*>(p.k_out) + t * p.k_stride + h * HD + e, vec, x);
-        else store8(static_cast<RT*>(p.v_out) + t * p.v_stride + h * HD + e, vec, x);
-        return;
-    }
+            const bool turn = p.rope && !is_v;
+            const bool some_pooled = __any_sync(0xffffffffu, in && pooled);
+            const RT* src = static_cast<const RT*>(is_k ? p.k : is_v ? p.v : p.q) + at;
+            RT* dst = static_cast<RT*>(p.q_out) + (first * p.q_out_stride + h * HD + e);
+            auto put = [&](int i, float (&x)[8]) {
+                if (i >= n || place[i] < 0) return;              // (the whole CTA: 4-bit pages take shuffles)
+                if (turn) {
+                    const float4 c0 = turns[i][0][tid % PER], c1 = turns[i][1][tid % PER];
+                    const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (good) {
-        const RT* src = static_cast<const RT*>(is_k ? p.k : is_v ? p.v : p.q) + t * (is_k ? p.k_stride : is_v ? p.v_stride : p.q_stride) + h * HD + e;
-        load8(src, vec, x);
-        if (!is_v && p.rope) {
-            float cs[8];
-            load8(p.rope + (size_t)pos * HD + e, vec, cs);
+                    for (int j = 0; j < 8; j += 2) {
+                        const float a = x[j], c = x[j + 1];
+                        x[j] = __fsub_rn(__fmul_rn(cs[j], a), __fmul_rn(cs[j + 1], c));
+                        x[j + 1] = __fadd_rn(__fmul_rn(cs[j + 1], a), __fmul_rn(cs[j], c));
+                    }
+                }
+                const long long row = pool_row[i];
+                if constexpr (Q4) {
+                    if (some_pooled) {
+                        // two neighbouring threads hold the 16 values of a scale
+                        float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float a = x[j], c = x[j + 1];
-                x[j] = __fsub_rn(__fmul_rn(cs[j], a), __fmul_rn(cs[j + 1], c));
-                x[j + 1] = __fadd_rn(__fmul_rn(cs[j + 1], a), __fmul_rn(cs[j], c));
+                        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        if (in && pooled && row >= 0) {
+                            const unsigned char s = f32_to_e4m3(__fdiv_rn(top, __fmul_rn(6.f, g)));
+                            const float unit = __fmul_rn(e4m3_to_f32(s), g), inv = unit > 0.f ? __fdiv_rn(1.f, unit) : 0.f;
+                            float y[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[j], inv);
+                            *reinterpret_cast<uint32_t*>(pool + row * (HD / 2)) = f32x8_to_e2m1(y);
+                            if (e % 16 == 0) scales[row * (HD / 16)] = s;
+                        }
+                    }
+                } else if (in && pooled && row >= 0) {
+                    store8(reinterpret_cast<KVT*>(pool) + row * HD, true, x);
+                }
+                if (in && !pooled) store8(dst + i * p.q_out_stride, vec, x);
+            };
+            // several rows at a time, so that the loads of all are on their way
+            constexpr int U = 8 / sizeof(RT);
+            for (int i = 0; i < n; i += U) {
+                Raw8<RT> raw[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i + u >= n || place[i + u] < 0 || !in) continue;
+                    raw[u].load(src + (i + u) * stride, vec);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float x[8];
+                    raw[u].get(x);
+                    put(i + u, x);
+                }
             }
         }
     }
-    if constexpr (sizeof(KVT) == 1) {
-        // two neighbouring threads hold the 16 values of a scale
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        if (good && (is_k || is_v)) {
-            const float g = is_k ? p.c.k_scale : p.c.v_scale;
-            const unsigned char s = f32_to_e4m3(__fdiv_rn(top, __fmul_rn(6.f, g)));
-            const float unit = __fmul_rn(e4m3_to_f32(s), g), inv = unit > 0.f ? __fdiv_rn(1.f, unit) : 0.f;
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[j], inv);
-            *reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(is_k ? p.c.kpool : p.c.vpool) + row * (HD / 2) + e / 2) = f32x8_to_e2m1(y);
-            if (e % 16 == 0) (is_k ? p.c.kscale : p.c.vscale)[row * (HD / 16) + e / 16] = s;
-        }
-    } else if (good && (is_k || is_v)) {
-        store8(static_cast<KVT*>(is_k ? p.c.kpool : p.c.vpool) + row * HD + e, true, x);
-    }
-    if (good && !is_k && !is_v) store8(static_cast<RT*>(p.q_out) + t * p.q_out_stride + h * HD + e, vec, x);
 }
 
 template <bool READ, typename KVT, typename RT>
-cudaError_t move_launch(const MoveParams& p, int hd, cudaStream_t st) {
-    const long long units = (long long)p.r.rows * (2 * p.c.kv_heads + (READ ? 0 : p.heads)) * (hd / 8);
-    const long long ctas = (units + kMoveThreads - 1) / kMoveThreads;
-    if (hd == 64) kv_move_kernel<KVT, RT, 64, READ><<<(unsigned)ctas, kMoveThreads, 0, st>>>(p);
-    else kv_move_kernel<KVT, RT, 128, READ><<<(unsigned)ctas, kMoveThreads, 0, st>>>(p);
+cudaError_t move_launch(MoveParams p, int hd, int sm_count, cudaStream_t st) {
+    // threads for the heads of a row, or a part of them; more rows of a CTA where there are enough for eight CTAs on each SM
+    const int units = (2 * p.c.kv_heads + (READ ? 0 : p.heads)) * (hd / 8);
+    const int threads = std::min(kMoveThreads, (units + 31) / 32 * 32);
+    p.cta_rows = std::max(1, std::min(kMoveRows, p.r.rows / (8 * sm_count)));
+    const unsigned ctas = (unsigned)((p.r.rows + p.cta_rows - 1) / p.cta_rows);
+    if (hd == 64) kv_move_kernel<KVT, RT, 64, READ><<<ctas, threads, 0, st>>>(p);
+    else kv_move_kernel<KVT, RT, 128, READ><<<ctas, threads, 0, st>>>(p);
     return cudaGetLastError();
 }
 template <bool READ>
-cudaError_t move_types(const MoveParams& p, int dtype, int row_dtype, int hd, cudaStream_t st) {
+cudaError_t move_types(const MoveParams& p, int dtype, int row_dtype, int hd, int sm_count, cudaStream_t st) {
     const bool f = row_dtype == MLB_DT_F32;
-    if (dtype == MLB_DT_F32) return f ? move_launch<READ, float, float>(p, hd, st) : move_launch<READ, float, bf16_t>(p, hd, st);
-    if (dtype == MLB_DT_BF16) return f ? move_launch<READ, bf16_t, float>(p, hd, st) : move_launch<READ, bf16_t, bf16_t>(p, hd, st);
-    return f ? move_launch<READ, fp4_t, float>(p, hd, st) : move_launch<READ, fp4_t, bf16_t>(p, hd, st);
+    if (dtype == MLB_DT_F32) return f ? move_launch<READ, float, float>(p, hd, sm_count, st) : move_launch<READ, float, bf16_t>(p, hd, sm_count, st);
+    if (dtype == MLB_DT_BF16) return f ? move_launch<READ, bf16_t, float>(p, hd, sm_count, st) : move_launch<READ, bf16_t, bf16_t>(p, hd, sm_count, st);
+    return f ? move_launch<READ, fp4_t, float>(p, hd, sm_count, st) : move_launch<READ, fp4_t, bf16_t>(p, hd, sm_count, st);
 }
 
 bool on16(const void* p, int64_t stride, int elt) { return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)stride * elt) & 15) == 0; }
@@ -369,7 +426,7 @@ extern "C" int mlb_op_kv_append(mlb_ops* o, const mlb_paged_kv* kv, const mlb_ne
     }
     OnDevice on(o->device);
     CU(on.err);
-    CU(move_types<false>(p, kv->dtype, row_dtype, kv->head_dim, static_cast<cudaStream_t>(stream)));
+    CU(move_types<false>(p, kv->dtype, row_dtype, kv->head_dim, o->sm_count, static_cast<cudaStream_t>(stream)));
     return MLB_OK;
 }
 
@@ -390,7 +447,7 @@ extern "C" int mlb_op_kv_read(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_
     p.vec = on16(k_out, k_stride, elt) && on16(v_out, v_stride, elt);
     OnDevice on(o->device);
     CU(on.err);
-    CU(move_types<true>(p, kv->dtype, row_dtype, kv->head_dim, static_cast<cudaStream_t>(stream)));
+    CU(move_types<true>(p, kv->dtype, row_dtype, kv->head_dim, o->sm_count, static_cast<cudaStream_t>(stream)));
     return MLB_OK;
 }
 
