@@ -25,7 +25,7 @@ template <typename KVT> constexpr int kPpTiles = sizeof(KVT) == 1 ? 2 : 1;
 constexpr int kPpKeys = 128;                     // positions of a step
 constexpr int kPpPages = kPpKeys / kKvBlock;
 template <typename KVT> constexpr int kPpLoaders = sizeof(KVT) == 1 ? 4 : 1;                             // warps that bring K and V
-template <typename KVT> constexpr int kPpThreads = 128 * kPpTiles<KVT> + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
+template <typename KVT> constexpr int kPpThreads = 256 * kPpTiles<KVT> + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
 constexpr float kPpLazy = 8.f;
 constexpr uint32_t kPpSpin = 1u << 24;
 
@@ -39,15 +39,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
         : "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-        "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
-        "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
-        : "memory");
-}
 // The registers of loads that tmem_ld_wait() has waited for: no use of them is moved before it
 __device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
     asm volatile(""
@@ -56,12 +47,24 @@ __device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
                    "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
                    "+r"(r[31]));
 }
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[16]) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
                  "r"(r[14]), "r"(r[15]), "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr)
                  : "memory");
 }
 // Largest of three; a NaN if one of them is
@@ -72,11 +75,11 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 }
 // 2^x of two numbers, x <= 128, without the exponential's unit: x = n + r with n the nearest whole number, 2^r by the cubic 1 + r (a + r (b + r c))
 // whose largest relative error over -1/2 .. 1/2 is smallest (fitted by reweighted least squares: 1.0e-4, a twentieth of the half step of bf16
-// that the weight is rounded by next), n added to the exponent. Below 2^-126: about that.
+// that the weight is rounded by next), n added to the exponent. Below 2^-126: something below that, and exactly 0 from 2^-127 on.
 __device__ __forceinline__ f32x2 ex2_poly(f32x2 x) {
     float a, d;
     unpack2(x, a, d);
-    x = pack2(fmaxf(a, -126.f), fmaxf(d, -126.f));
+    x = pack2(fmaxf(a, -127.f), fmaxf(d, -127.f));
     const float big = 12582912.f;                // 1.5 * 2^23: whole numbers are its low bits
     const f32x2 n = add2(x, pack2(big, big)), r = fma2(add2(n, pack2(-big, -big)), pack2(-1.f, -1.f), x);
     f32x2 y = fma2(pack2(0.05500893f, 0.05500893f), r, pack2(0.24221100f, 0.24221100f));
@@ -141,7 +144,7 @@ struct PromptSmem {
     static constexpr uint32_t kQ = 128 * HD * 2, kKV = kPpKeys * HD * 2, kHalf = 128 * 128;      // bytes of a tile; of 64 dims of one
     static constexpr uint32_t q = 0, k = TILES * kQ, v = k + stages * kKV, bars = v + stages * kKV, total = bars + 256;
 };
-enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_COUNT = 17 };
+enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_END = 17, PB_COUNT = 18 };
 
 // 4-bit pages: eight codes (dims 0 .. 7) -> four bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code * scale / 256. Exponent and mantissa of
 // a code are put at the low end of a bf16's exponent, which makes it code * 2^-126 exactly (0.5 as a subnormal), and multiplied by `s`, the
@@ -171,9 +174,11 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     __shared__ uint32_t tmem_base;
     __shared__ int found[5];                     // sequence, tile in it, the sequence's first row, rows, positions
+    __shared__ float shared_row[TILES][2][128];  // of a row's two threads: maxima, then sums
+    __shared__ unsigned odd_rows[TILES][2][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr bool Q4 = sizeof(KVT) == 1;
-    constexpr int kLoader = 4 * TILES, kIssuer = kLoader + kPpLoaders<KVT>;
+    constexpr int kLoader = 8 * TILES, kIssuer = kLoader + kPpLoaders<KVT>;
 
     if (warp == kIssuer) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256u * TILES) : "memory");
@@ -182,13 +187,13 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     }
     if (warp == kLoader) {
         // which sequence's rows these are: those of sequences with more than kSplitRows, 128 TILES at a time, later rows (which see more) first
-        int want = (int)(gridDim.x - 1 - blockIdx.x), at = -1;
+        int want = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)p.c.kv_heads), at = -1;
         for (int b0 = 0; b0 < p.r.batch && at < 0; b0 += 32) {
             const int b = b0 + lane;
             int n = 0;
             PagedSeq s = {0, 0, 0};
             if (b < p.r.batch) {
-                s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0 && blockIdx.y == 0);
+                s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0);
                 const long long rows = (long long)s.n * p.group;
                 n = rows > kSplitRows ? (int)((rows + 128 * TILES - 1) / (128 * TILES)) : 0;
             }
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             found[1] = want;
             for (int i = 0; i < PB_COUNT; ++i) {
                 const bool filled = i == PB_KFULL || i == PB_KFULL + 1 || i == PB_VFULL || i == PB_VFULL + 1;
-                mbar_init(bar(i), i == PB_Q ? 128 * TILES : (i >= PB_P && i < PB_O) || (Q4 && filled) ? 128 : 1);
+                mbar_init(bar(i), i == PB_Q ? 8 * TILES : i >= PB_P && i < PB_O ? 8 : Q4 && filled ? 128 : 1);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         if (warp == kIssuer) release();
         return;
     }
-    const int b = found[0], kvh = blockIdx.y, first = found[1] * 128 * TILES;
+    const int b = found[0], kvh = (int)((gridDim.x - 1 - blockIdx.x) % (unsigned)p.c.kv_heads), first = found[1] * 128 * TILES;
     const PagedSeq s = {found[2], found[3], found[4]};
     const int count = min(128 * TILES, s.n * p.group - first), tiles = TILES == 2 && count > 128 ? 2 : 1;
     const int pos0 = s.len - s.n, low = pos0 + first / p.group, high = pos0 + (first + count - 1) / p.group;
@@ -294,6 +299,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         }
     } else if (!Q4 && warp == kLoader) {
         bool good = true;
+        int filled[2] = {0, 0};                  // steps whose K, V are on their way or there
         for (int j = 0; j < steps && good; ++j) {
             const int st = j % NST;
             const uint32_t ph = (uint32_t)(j / NST) & 1u;
@@ -313,6 +319,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 for (int h = 0; h < HD / 64; ++h)
                     tma_load_2d(sm0 + L::k + st * L::kKV + h * L::kHalf + lane * 2048, &tmK, h * 64, row0, bar(PB_KFULL + st));
             }
+            filled[0] = j + 1;
             good = __all_sync(0xffffffffu, wait(PB_VEMPTY + st, ph ^ 1u));
             if (!good) break;
             for (unsigned left = by_hand; left; left &= left - 1) {
@@ -335,6 +342,11 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 for (int h = 0; h < HD / 64; ++h)
                     tma_load_2d(sm0 + L::v + st * L::kKV + h * L::kHalf + lane * 2048, &tmV, h * 64, row0, bar(PB_VFULL + st));
             }
+            filled[1] = j + 1;
+        }
+        if (!good) {                             // no copy outlives the CTA
+            for (int i = 0; i < 2; ++i)
+                for (int j = max(0, filled[i] - NST); j < filled[i]; ++j) wait((i ? PB_VFULL : PB_KFULL) + j % NST, (uint32_t)(j / NST) & 1u);
         }
     } else if (warp == kIssuer) {
         if (steps > 0) {
@@ -361,14 +373,16 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                     if (!good) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < kPpKeys / 16; ++ks) {
-                        if (ks == kPpKeys / 32) {
+                    for (int i = 0; i < kPpKeys / 16; ++i) {
+                        // weights lie where the scores of their half were; those of each half's first 32 positions come first
+                        const int ks = (i & 1) + (i & 2) * 2 + (i & 4) / 2;
+                        if (i == kPpKeys / 32) {
                             good = all_wait(PB_P2 + t, (uint32_t)j & 1u);
                             if (!good) break;
                             tc_fence_after();
                         }
-                        umma_ts(tmem + (TILES + t) * 128, tmem + t * 128 + ks * 8, umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
-                                     j > 0 || ks > 0);
+                        umma_ts(tmem + (TILES + t) * 128, tmem + t * 128 + ks / 4 * 64 + ks % 4 * 8, umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
+                                     j > 0 || i > 0);
                     }
                     if (!good) break;
                     if (t == tiles - 1) commit_elected(bar(PB_VEMPTY + j % NST));
@@ -385,114 +399,163 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                     }
                 }
             }
+            if (!good) {                         // nor does a product
+                commit_elected(bar(PB_END));
+                all_wait(PB_END, 0);
+            }
         }
     } else {
-        const int t = warp / 4, r = tid & 127, i = t * 128 + r;      // this thread's row of the CTA's
+        // Two threads of a row, for 64 of the step's positions each: their warps, four apart, share the row's 32 lanes of tensor memory. With one
+        // thread for all 128 a step's maximum and exponentials took 2200 cycles, twice the tile's products, and an SM's 8 such warps did not hide them.
+        const int t = warp / 8, half = warp / 4 & 1, r = tid & 127, i = t * 128 + r;      // this thread's row of the CTA's
         const bool in = i < count;
         const int rr = first + (in ? i : 0), row = s.r0 + rr / p.group, h = kvh * p.group + rr % p.group;
         const int pos = in ? pos0 + rr / p.group : high;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // the warp's 32 lanes of tensor memory
-        // the row's queries, K-major with the swizzle that the MMA expects; a negative scale turns their sign
+        const int pair = 1 + t * 4 + (warp & 3);                      // named barrier of the two warps of these rows
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
+        auto pair_any = [&](bool x) {
+            uint32_t y;
+            asm volatile(
+                "{\n"
+                ".reg .pred a, b;\n"
+                "setp.ne.u32 a, %1, 0;\n"
+                "bar.red.or.pred b, %2, 64, a;\n"
+                "selp.u32 %0, 1, 0, b;\n"
+                "}\n"
+                : "=r"(y)
+                : "r"((uint32_t)x), "r"(pair)
+                : "memory");
+            return y != 0;
+        };
+        // The tile's rows lie in memory by (token, head); a warp takes 16 of them, and CH lanes the 16-byte pieces of one, so that it reads and writes
+        // whole rows: `piece(k)` is the k-th of a lane. (A row per thread: 4 us for the queries and 3 for the results.)
+        constexpr int CH = HD / 8, NP = 16 * CH / 32;
+        struct Piece { int r, c; bool in; long long row, col; };
+        auto piece = [&](int k) {
+            Piece x;
+            x.r = (warp & 3) * 32 + half * 16 + k * (32 / CH) + lane / CH;
+            x.c = lane % CH;
+            x.in = t * 128 + x.r < count;
+            const int a = first + (x.in ? t * 128 + x.r : 0), token = a / p.group;
+            x.row = s.r0 + token;
+            x.col = (long long)(kvh * p.group + a - token * p.group) * HD + x.c * 8;
+            return x;
+        };
+        auto staged = [&](int rl, int ch) { return reinterpret_cast<uint4*>(sm + L::q + t * L::kQ + ch / 8 * L::kHalf + rl * 128 + ((ch % 8) ^ (rl & 7)) * 16); };
+        // queries, K-major with the swizzle that the MMA expects; a negative scale turns their sign
         const float scale = p.scale * p.c.k_scale * (Q4 ? kPpCodeScale : 1.f) * 1.4426950408889634f;
         {
-            const bf16_t* q = static_cast<const bf16_t*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD;
-            const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+            const bf16_t* q = static_cast<const bf16_t*>(p.q);
+            const bool vec = ((reinterpret_cast<uintptr_t>(q) | (uint64_t)p.q_stride * 2) & 15) == 0;
             const uint32_t turn = scale < 0.f ? 0x80008000u : 0u;
+            uint4 x[NP];
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (in) {
-                    if (vec) {
-                        x = __ldg(reinterpret_cast<const uint4*>(q) + c);
-                    } else {
-                        uint32_t w[4];
+            for (int k = 0; k < NP; ++k) {
+                const Piece y = piece(k);
+                const bf16_t* src = q + y.row * p.q_stride + y.col;
+                x[k] = make_uint4(0, 0, 0, 0);
+                if (y.in && vec) x[k] = __ldg(reinterpret_cast<const uint4*>(src));
+                if (y.in && !vec) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = (uint32_t)__bfloat16_as_ushort(q[c * 8 + 2 * e]) | (uint32_t)__bfloat16_as_ushort(q[c * 8 + 2 * e + 1]) << 16;
-                        x = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    x.x ^= turn; x.y ^= turn; x.z ^= turn; x.w ^= turn;
-                    if (Q4)                                      // the order of dims in K
-                        x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+                    for (int e = 0; e < 4; ++e) w[e] = (uint32_t)__bfloat16_as_ushort(src[2 * e]) | (uint32_t)__bfloat16_as_ushort(src[2 * e + 1]) << 16;
+                    x[k] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                *reinterpret_cast<uint4*>(sm + L::q + t * L::kQ + c / 8 * L::kHalf + r * 128 + ((c % 8) ^ (r & 7)) * 16) = x;
+            }
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                uint4 v = x[k];
+                v.x ^= turn; v.y ^= turn; v.z ^= turn; v.w ^= turn;
+                if (Q4)                                          // the order of dims in K
+                    v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+                const Piece y = piece(k);
+                *staged(y.r, y.c) = y.in ? v : make_uint4(0, 0, 0, 0);
             }
             fence_async_smem();
-            mbar_arrive(bar(PB_Q));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(PB_Q));
         }
         const float c = fabsf(scale);
         float m = -INFINITY, l = 0.f;
-        bool good = true;
+        bool good = true;                        // (a warp whose wait ran out goes on without waiting: its partner's barriers need it)
         if (t < tiles) {
             const int wlow = __reduce_min_sync(0xffffffffu, pos), whigh = __reduce_max_sync(0xffffffffu, pos);
+            const uint32_t sc = tmem + lanes + t * 128 + half * 64;
             for (int j = 0; j < steps; ++j) {
-                good = __all_sync(0xffffffffu, wait(PB_S + t, (uint32_t)j & 1u));
-                if (!good) break;
+                good = good && __all_sync(0xffffffffu, wait(PB_S + t, (uint32_t)j & 1u));
                 tc_fence_after();
+                uint32_t x[2][32];
+                tmem_ld32(sc, x[0]);
+                tmem_ld32(sc + 32, x[1]);
                 // positions that some row of the warp does not see
-                bool edge = (j + 1) * kPpPages > span.count;
+                const int v0 = j * kPpPages + half * (kPpPages / 2);
+                bool edge = v0 + kPpPages / 2 > span.count;
                 if (!edge) {
-                    const int ka = span.page(j * kPpPages) * kKvBlock, kb = span.page(j * kPpPages + kPpPages - 1) * kKvBlock + kKvBlock - 1;
+                    const int ka = span.page(v0) * kKvBlock, kb = span.page(v0 + kPpPages / 2 - 1) * kKvBlock + kKvBlock - 1;
                     edge = kb > wlow || (p.window > 0 && ka <= whigh - p.window && !(kb < p.sinks));
                 }
-                // 32 positions from 32 g on: those that the row does not see to -inf
-                auto hide = [&](uint32_t (&x)[32], int g) {
+                tmem_ld_wait();
+                tmem_loaded(x[0]);
+                tmem_loaded(x[1]);
+                if (edge) {                                      // those that the row does not see to -inf
+                    auto below = [](int n) { return (1u << min(max(n, 0), kKvBlock)) - 1u; };
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int v = j * kPpPages + 2 * g + u, k0 = v < span.count ? span.page(v) * kKvBlock : 0x40000000;
-                        const int hi = pos - k0, lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) - k0, sk = p.sinks - k0;
+                    for (int g = 0; g < 2; ++g) {
+                        uint32_t seen = 0;
 #pragma unroll
-                        for (int e = 0; e < kKvBlock; ++e)
-                            if (!(e <= hi && (e >= lo || e < sk))) x[u * kKvBlock + e] = 0xff800000u;
+                        for (int u = 0; u < 2; ++u) {
+                            const int v = v0 + 2 * g + u;
+                            if (v < span.count) {
+                                const int k0 = span.page(v) * kKvBlock, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+                                seen |= (below(pos + 1 - k0) & (~below(lo - k0) | below(p.sinks - k0))) << (u * kKvBlock);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(seen >> e & 1u)) x[g][e] = 0xff800000u;
                     }
-                };
-                const uint32_t sc = tmem + lanes + t * 128;
-                // The scores are read twice, for the maximum and for the weights: held in between, 128 registers of a thread would be theirs.
-                float mx;
-                {
-                    uint32_t x[2][32];
-                    float top[2] = {-INFINITY, -INFINITY};
-                    tmem_ld32(sc, x[0]);
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        tmem_ld_wait();
-                        tmem_loaded(x[g & 1]);
-                        if (g < 3) tmem_ld32(sc + 32 * (g + 1), x[(g + 1) & 1]);
-                        if (edge) hide(x[g & 1], g);
-#pragma unroll
-                        for (int u = 0; u < 32; u += 2)
-                            top[u / 2 & 1] = max3_nan(top[u / 2 & 1], __uint_as_float(x[g & 1][u]), __uint_as_float(x[g & 1][u + 1]));
-                    }
-                    mx = max3_nan(top[0], top[1], -INFINITY) * c;
                 }
-                const bool moved = !(mx <= m + kPpLazy);      // (a score that is no number makes the maximum, and so the row, none)
-                if (__any_sync(0xffffffffu, moved)) {
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int u = 0; u < 64; u += 2)
+                    top[u / 2 & 1] = max3_nan(top[u / 2 & 1], __uint_as_float(x[u / 32][u % 32]), __uint_as_float(x[u / 32][u % 32 + 1]));
+                float mx = max3_nan(top[0], top[1], -INFINITY) * c;
+                // (a score that is no number makes the maximum, and so the row, none)
+                if (pair_any(!(mx <= m + kPpLazy))) {
+                    shared_row[t][half][r] = mx;
+                    pair_sync();
+                    mx = max3_nan(mx, shared_row[t][half ^ 1][r], -INFINITY);
+                    const bool moved = !(mx <= m + kPpLazy);
                     const float f = moved ? ex2(m - mx) : 1.f;
                     if (moved) m = mx;
                     l *= f;
                     if (j > 0) {
 #pragma unroll 1
-                        for (int e = 0; e < HD / 32; ++e) {
-                            uint32_t o[32];
-                            tmem_ld32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
+                        for (int e = half * (HD / 32); e < (half + 1) * (HD / 32); ++e) {
+                            uint32_t o[16];
+                            const uint32_t at = tmem + lanes + (TILES + t) * 128 + e * 16;
+                            tmem_ld16(at, o);
                             tmem_ld_wait();
                             tmem_loaded(o);
 #pragma unroll
-                            for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
-                            tmem_st32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
+                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                            tmem_st16(at, o);
                         }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
                 const f32x2 cc = pack2(c, c), rr2 = pack2(-ref, -ref);
                 f32x2 sum[2] = {0ull, 0ull};
-                // weights of 32 positions, one pair of four by polynomial: the exponential's unit takes 16 a cycle and would be the bound
-                auto weigh = [&](auto by_unit, const uint32_t (&x)[32], uint32_t (&w)[16]) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    // weights of 32 positions, one pair of four by polynomial: the exponential's unit takes 16 a cycle and would be the bound
+                    uint32_t w[16];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) {
-                        f32x2 y = fma2(pack2u(x[2 * u], x[2 * u + 1]), cc, rr2);
+                        f32x2 y = fma2(pack2u(x[g][2 * u], x[g][2 * u + 1]), cc, rr2);
                         float a, d;
-                        if (!decltype(by_unit)::value && u % 4 == 3) {
+                        if (u % 4 == 3) {
                             y = ex2_poly(y);
                             unpack2(y, a, d);
                         } else {
@@ -504,28 +567,11 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                         sum[u & 1] = add2(sum[u & 1], y);
                         w[u] = f32x2_to_bf16(a, d);
                     }
-                };
-                {
-                    uint32_t x[2][32], w[16];
-                    tmem_ld32(sc, x[0]);
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        tmem_ld_wait();
-                        tmem_loaded(x[g & 1]);
-                        if (g < 3) tmem_ld32(sc + 32 * (g + 1), x[(g + 1) & 1]);
-                        if (edge) {
-                            hide(x[g & 1], g);
-                            weigh(std::true_type(), x[g & 1], w);      // exactly 0 where hidden
-                        } else {
-                            weigh(std::false_type(), x[g & 1], w);
-                        }
-                        tmem_st16(sc + 16 * g, w);               // over scores that have been read
-                        if (g & 1) {                             // half of the positions: their products can begin
-                            tmem_st_wait();
-                            tc_fence_before();
-                            mbar_arrive(bar((g == 1 ? PB_P : PB_P2) + t));
-                        }
-                    }
+                    tmem_st16(sc + 16 * g, w);                   // over scores that have been read
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar((g == 0 ? PB_P : PB_P2) + t));
                 }
                 float sa, sb, sd, se;
                 unpack2(sum[0], sa, sb);
@@ -533,17 +579,19 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 l += (sa + sb) + (sd + se);
             }
             // results
-            if (steps > 0 && good) {
-                good = __all_sync(0xffffffffu, wait(PB_O + t, 0));
+            if (steps > 0) {
+                good = good && __all_sync(0xffffffffu, wait(PB_O + t, 0));
                 tc_fence_after();
             }
+            pair_sync();                                         // the maxima have been read
+            shared_row[t][half][r] = l;
+            pair_sync();
+            l = shared_row[t][0][r] + shared_row[t][1][r];       // the same sum in both threads
+            const float inv = pos < 0 ? 0.f : p.c.v_scale * (Q4 ? kPpCodeScale : 1.f) / l;
+            bool odd = false;
             if (good) {
-                const float inv = pos < 0 ? 0.f : p.c.v_scale * (Q4 ? kPpCodeScale : 1.f) / l;
-                bool odd = false;
-                bf16_t* out = static_cast<bf16_t*>(p.out) + (size_t)row * p.out_stride + (size_t)h * HD;
-                const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll 1
-                for (int e = 0; e < HD / 32; ++e) {
+                for (int e = half * (HD / 64); e < (half + 1) * (HD / 64); ++e) {
                     uint32_t o[32];
                     if (steps > 0) {
                         tmem_ld32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
@@ -562,19 +610,39 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
 #pragma unroll
                         for (int u = 0; u < 32; ++u) y[u] *= gp[u];
                     }
-                    if (in) {
-                        if (vec) {
 #pragma unroll
-                            for (int u = 0; u < 32; u += 8)
-                                *reinterpret_cast<uint4*>(out + e * 32 + u) = make_uint4(f32x2_to_bf16(y[u], y[u + 1]), f32x2_to_bf16(y[u + 2], y[u + 3]),
-                                                                                         f32x2_to_bf16(y[u + 4], y[u + 5]), f32x2_to_bf16(y[u + 6], y[u + 7]));
-                        } else {
+                    for (int u = 0; u < 32; u += 8)              // where the queries were
+                        *staged(r, e * 4 + u / 8) = make_uint4(f32x2_to_bf16(y[u], y[u + 1]), f32x2_to_bf16(y[u + 2], y[u + 3]),
+                                                               f32x2_to_bf16(y[u + 4], y[u + 5]), f32x2_to_bf16(y[u + 6], y[u + 7]));
+                }
+            }
+            pair_sync();
+            if (good) {
+                bf16_t* out = static_cast<bf16_t*>(p.out);
+                const bool vec = ((reinterpret_cast<uintptr_t>(out) | (uint64_t)p.out_stride * 2) & 15) == 0;
 #pragma unroll
-                            for (int u = 0; u < 32; ++u) out[e * 32 + u] = __float2bfloat16_rn(y[u]);
+                for (int k = 0; k < NP; ++k) {
+                    const Piece y = piece(k);
+                    if (!y.in) continue;
+                    const uint4 v = *staged(y.r, y.c);
+                    bf16_t* dst = out + y.row * p.out_stride + y.col;
+                    if (vec) {
+                        *reinterpret_cast<uint4*>(dst) = v;
+                    } else {
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            dst[2 * e] = __ushort_as_bfloat16((unsigned short)(w[e] & 0xffffu));
+                            dst[2 * e + 1] = __ushort_as_bfloat16((unsigned short)(w[e] >> 16));
                         }
                     }
                 }
-                for (unsigned again = __ballot_sync(0xffffffffu, odd && in); again; again &= again - 1) {
+            }
+            const unsigned mine = __ballot_sync(0xffffffffu, odd && in && good);
+            if (lane == 0) odd_rows[t][half][warp & 3] = mine;
+            pair_sync();                                         // (what either warp has written is written)
+            if (half == 0) {
+                for (unsigned again = odd_rows[t][0][warp & 3] | odd_rows[t][1][warp & 3]; again; again &= again - 1) {
                     const int src = __ffs(again) - 1;
                     careful_row<KVT, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
                 }
@@ -602,7 +670,7 @@ cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st)
     cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<KVT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles<KVT>) + p.r.batch;
-    attn_prompt_kernel<KVT, HD><<<dim3((unsigned)tiles, p.c.kv_heads), kPpThreads<KVT>, smem, st>>>(tk, tv, p);
+    attn_prompt_kernel<KVT, HD><<<(unsigned)(tiles * p.c.kv_heads), kPpThreads<KVT>, smem, st>>>(tk, tv, p);
     return cudaGetLastError();
 }
 
