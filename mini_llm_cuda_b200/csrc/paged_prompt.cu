@@ -25,7 +25,11 @@ template <typename KVT> constexpr int kPpTiles = sizeof(KVT) == 1 ? 2 : 1;
 constexpr int kPpKeys = 128;                     // positions of a step
 constexpr int kPpPages = kPpKeys / kKvBlock;
 template <typename KVT> constexpr int kPpLoaders = sizeof(KVT) == 1 ? 4 : 1;                             // warps that bring K and V
-template <typename KVT> constexpr int kPpThreads = 256 * kPpTiles<KVT> + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
+// Threads of a row in the softmax. Two where TMA brings K and V: with one for all 128 positions a step's maximum and exponentials took 2200 cycles, twice
+// the tile's products, and 8 such warps on an SM did not hide them. One with 4-bit pages, whose loaders and softmax share the issue slots that bound them.
+template <typename KVT> constexpr int kPpHalves = sizeof(KVT) == 1 ? 1 : 2;
+template <typename KVT> constexpr int kPpThreads = 128 * kPpHalves<KVT> * kPpTiles<KVT> + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
+constexpr int kPpPoly = 4;                       // one pair of so many exponentials by polynomial
 constexpr float kPpLazy = 8.f;
 constexpr uint32_t kPpSpin = 1u << 24;
 
@@ -174,11 +178,12 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     __shared__ uint32_t tmem_base;
     __shared__ int found[5];                     // sequence, tile in it, the sequence's first row, rows, positions
-    __shared__ float shared_row[TILES][2][128];  // of a row's two threads: maxima, then sums
-    __shared__ unsigned odd_rows[TILES][2][4];
+    constexpr int HALVES = kPpHalves<KVT>, COLS = kPpKeys / HALVES;       // positions of a step for a softmax thread
+    __shared__ float shared_row[TILES][HALVES][128];      // of a row's two threads: maxima, then sums
+    __shared__ unsigned odd_rows[TILES][HALVES][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr bool Q4 = sizeof(KVT) == 1;
-    constexpr int kLoader = 8 * TILES, kIssuer = kLoader + kPpLoaders<KVT>;
+    constexpr int kLoader = 4 * HALVES * TILES, kIssuer = kLoader + kPpLoaders<KVT>;
 
     if (warp == kIssuer) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(256u * TILES) : "memory");
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             found[1] = want;
             for (int i = 0; i < PB_COUNT; ++i) {
                 const bool filled = i == PB_KFULL || i == PB_KFULL + 1 || i == PB_VFULL || i == PB_VFULL + 1;
-                mbar_init(bar(i), i == PB_Q ? 8 * TILES : i >= PB_P && i < PB_O ? 8 : Q4 && filled ? 128 : 1);
+                mbar_init(bar(i), i == PB_Q ? 4 * HALVES * TILES : i >= PB_P && i < PB_O ? 4 * HALVES : Q4 && filled ? 128 : 1);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -374,14 +379,14 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                     tc_fence_after();
 #pragma unroll
                     for (int i = 0; i < kPpKeys / 16; ++i) {
-                        // weights lie where the scores of their half were; those of each half's first 32 positions come first
-                        const int ks = (i & 1) + (i & 2) * 2 + (i & 4) / 2;
+                        // weights lie where the scores of their thread were; those of each thread's first positions come first
+                        const int ks = HALVES == 2 ? (i & 1) + (i & 2) * 2 + (i & 4) / 2 : i;
                         if (i == kPpKeys / 32) {
                             good = all_wait(PB_P2 + t, (uint32_t)j & 1u);
                             if (!good) break;
                             tc_fence_after();
                         }
-                        umma_ts(tmem + (TILES + t) * 128, tmem + t * 128 + ks / 4 * 64 + ks % 4 * 8, umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
+                        umma_ts(tmem + (TILES + t) * 128, tmem + t * 128 + (HALVES == 2 ? ks / 4 * 64 + ks % 4 * 8 : ks * 8), umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
                                      j > 0 || i > 0);
                     }
                     if (!good) break;
@@ -405,16 +410,19 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             }
         }
     } else {
-        // Two threads of a row, for 64 of the step's positions each: their warps, four apart, share the row's 32 lanes of tensor memory. With one
-        // thread for all 128 a step's maximum and exponentials took 2200 cycles, twice the tile's products, and an SM's 8 such warps did not hide them.
-        const int t = warp / 8, half = warp / 4 & 1, r = tid & 127, i = t * 128 + r;      // this thread's row of the CTA's
+        // The warps of a row's two threads, four apart, share its 32 lanes of tensor memory.
+        const int t = warp / (4 * HALVES), half = HALVES == 2 ? warp / 4 & 1 : 0, r = tid & 127, i = t * 128 + r;      // this thread's row of the CTA's
         const bool in = i < count;
         const int rr = first + (in ? i : 0), row = s.r0 + rr / p.group, h = kvh * p.group + rr % p.group;
         const int pos = in ? pos0 + rr / p.group : high;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // the warp's 32 lanes of tensor memory
         const int pair = 1 + t * 4 + (warp & 3);                      // named barrier of the two warps of these rows
-        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
+        auto pair_sync = [&]() {
+            if constexpr (HALVES == 2) asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+            else __syncwarp();
+        };
         auto pair_any = [&](bool x) {
+            if constexpr (HALVES == 1) return __any_sync(0xffffffffu, x) != 0;
             uint32_t y;
             asm volatile(
                 "{\n"
@@ -428,13 +436,13 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 : "memory");
             return y != 0;
         };
-        // The tile's rows lie in memory by (token, head); a warp takes 16 of them, and CH lanes the 16-byte pieces of one, so that it reads and writes
+        // The tile's rows lie in memory by (token, head); a warp takes 16 or 32 of them, and CH lanes the 16-byte pieces of one, so that it reads and writes
         // whole rows: `piece(k)` is the k-th of a lane. (A row per thread: 4 us for the queries and 3 for the results.)
-        constexpr int CH = HD / 8, NP = 16 * CH / 32;
+        constexpr int CH = HD / 8, NP = 32 / HALVES * CH / 32;
         struct Piece { int r, c; bool in; long long row, col; };
         auto piece = [&](int k) {
             Piece x;
-            x.r = (warp & 3) * 32 + half * 16 + k * (32 / CH) + lane / CH;
+            x.r = (warp & 3) * 32 + half * (32 / HALVES) + k * (32 / CH) + lane / CH;
             x.c = lane % CH;
             x.in = t * 128 + x.r < count;
             const int a = first + (x.in ? t * 128 + x.r : 0), token = a / p.group;
@@ -449,10 +457,12 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             const bf16_t* q = static_cast<const bf16_t*>(p.q);
             const bool vec = ((reinterpret_cast<uintptr_t>(q) | (uint64_t)p.q_stride * 2) & 15) == 0;
             const uint32_t turn = scale < 0.f ? 0x80008000u : 0u;
-            uint4 x[NP];
+            constexpr int NQ = NP < 8 ? NP : 8;                  // loads on their way at once
+            for (int k0 = 0; k0 < NP; k0 += NQ) {
+            uint4 x[NQ];
 #pragma unroll
-            for (int k = 0; k < NP; ++k) {
-                const Piece y = piece(k);
+            for (int k = 0; k < NQ; ++k) {
+                const Piece y = piece(k0 + k);
                 const bf16_t* src = q + y.row * p.q_stride + y.col;
                 x[k] = make_uint4(0, 0, 0, 0);
                 if (y.in && vec) x[k] = __ldg(reinterpret_cast<const uint4*>(src));
@@ -464,13 +474,14 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 }
             }
 #pragma unroll
-            for (int k = 0; k < NP; ++k) {
+            for (int k = 0; k < NQ; ++k) {
                 uint4 v = x[k];
                 v.x ^= turn; v.y ^= turn; v.z ^= turn; v.w ^= turn;
                 if (Q4)                                          // the order of dims in K
                     v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-                const Piece y = piece(k);
+                const Piece y = piece(k0 + k);
                 *staged(y.r, y.c) = y.in ? v : make_uint4(0, 0, 0, 0);
+            }
             }
             fence_async_smem();
             __syncwarp();
@@ -481,58 +492,68 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         bool good = true;                        // (a warp whose wait ran out goes on without waiting: its partner's barriers need it)
         if (t < tiles) {
             const int wlow = __reduce_min_sync(0xffffffffu, pos), whigh = __reduce_max_sync(0xffffffffu, pos);
-            const uint32_t sc = tmem + lanes + t * 128 + half * 64;
+            const uint32_t sc = tmem + lanes + t * 128 + half * COLS;
+            // Scores: two threads of a row hold theirs in registers, one reads them twice, for the maximum and for the weights.
+            constexpr int NG = COLS / 32;
+            uint32_t x[2][32];
             for (int j = 0; j < steps; ++j) {
                 good = good && __all_sync(0xffffffffu, wait(PB_S + t, (uint32_t)j & 1u));
                 tc_fence_after();
-                uint32_t x[2][32];
                 tmem_ld32(sc, x[0]);
-                tmem_ld32(sc + 32, x[1]);
+                if (HALVES == 2) tmem_ld32(sc + 32, x[1]);
                 // positions that some row of the warp does not see
                 const int v0 = j * kPpPages + half * (kPpPages / 2);
-                bool edge = v0 + kPpPages / 2 > span.count;
+                bool edge = v0 + kPpPages / HALVES > span.count;
                 if (!edge) {
-                    const int ka = span.page(v0) * kKvBlock, kb = span.page(v0 + kPpPages / 2 - 1) * kKvBlock + kKvBlock - 1;
+                    const int ka = span.page(v0) * kKvBlock, kb = span.page(v0 + kPpPages / HALVES - 1) * kKvBlock + kKvBlock - 1;
                     edge = kb > wlow || (p.window > 0 && ka <= whigh - p.window && !(kb < p.sinks));
                 }
-                tmem_ld_wait();
-                tmem_loaded(x[0]);
-                tmem_loaded(x[1]);
-                if (edge) {                                      // those that the row does not see to -inf
+                // 32 positions from 32 g on: those that the row does not see to -inf
+                auto hide = [&](uint32_t (&y)[32], int g) {
                     auto below = [](int n) { return (1u << min(max(n, 0), kKvBlock)) - 1u; };
+                    uint32_t seen = 0;
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        uint32_t seen = 0;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int v = v0 + 2 * g + u;
-                            if (v < span.count) {
-                                const int k0 = span.page(v) * kKvBlock, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-                                seen |= (below(pos + 1 - k0) & (~below(lo - k0) | below(p.sinks - k0))) << (u * kKvBlock);
-                            }
+                    for (int u = 0; u < 2; ++u) {
+                        const int v = v0 + 2 * g + u;
+                        if (v < span.count) {
+                            const int k0 = span.page(v) * kKvBlock, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+                            seen |= (below(pos + 1 - k0) & (~below(lo - k0) | below(p.sinks - k0))) << (u * kKvBlock);
                         }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(seen >> e & 1u)) x[g][e] = 0xff800000u;
                     }
-                }
-                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int u = 0; u < 64; u += 2)
-                    top[u / 2 & 1] = max3_nan(top[u / 2 & 1], __uint_as_float(x[u / 32][u % 32]), __uint_as_float(x[u / 32][u % 32 + 1]));
-                float mx = max3_nan(top[0], top[1], -INFINITY) * c;
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen >> e & 1u)) y[e] = 0xff800000u;
+                };
+                auto arrived = [&](int g) {                      // scores of group g are in x[g & 1], and the next ones on their way
+                    if (HALVES == 1 || g == 0) tmem_ld_wait();
+                    if (HALVES == 2 && g == 0) tmem_loaded(x[1]);
+                    if (HALVES == 1 || g == 0) tmem_loaded(x[g & 1]);
+                    if (HALVES == 1 && g + 1 < NG) tmem_ld32(sc + 32 * (g + 1), x[(g + 1) & 1]);
+                    if (edge) hide(x[g & 1], g);
+                };
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    arrived(g);
+#pragma unroll
+                    for (int u = 0; u < 32; u += 2)
+                        top[u / 2 & 3] = max3_nan(top[u / 2 & 3], __uint_as_float(x[g & 1][u]), __uint_as_float(x[g & 1][u + 1]));
+                }
+                float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], -INFINITY) * c;
                 // (a score that is no number makes the maximum, and so the row, none)
                 if (pair_any(!(mx <= m + kPpLazy))) {
-                    shared_row[t][half][r] = mx;
-                    pair_sync();
-                    mx = max3_nan(mx, shared_row[t][half ^ 1][r], -INFINITY);
+                    if constexpr (HALVES == 2) {
+                        shared_row[t][half][r] = mx;
+                        pair_sync();
+                        mx = max3_nan(mx, shared_row[t][half ^ 1][r], -INFINITY);
+                    }
                     const bool moved = !(mx <= m + kPpLazy);
                     const float f = moved ? ex2(m - mx) : 1.f;
                     if (moved) m = mx;
                     l *= f;
                     if (j > 0) {
 #pragma unroll 1
-                        for (int e = half * (HD / 32); e < (half + 1) * (HD / 32); ++e) {
+                        for (int e = half * (HD / 16 / HALVES); e < (half + 1) * (HD / 16 / HALVES); ++e) {
                             uint32_t o[16];
                             const uint32_t at = tmem + lanes + (TILES + t) * 128 + e * 16;
                             tmem_ld16(at, o);
@@ -547,15 +568,17 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 const float ref = m == -INFINITY ? 0.f : m;
                 const f32x2 cc = pack2(c, c), rr2 = pack2(-ref, -ref);
                 f32x2 sum[2] = {0ull, 0ull};
+                if (HALVES == 1) tmem_ld32(sc, x[0]);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
+                for (int g = 0; g < NG; ++g) {
+                    if (HALVES == 1) arrived(g);
                     // weights of 32 positions, one pair of four by polynomial: the exponential's unit takes 16 a cycle and would be the bound
                     uint32_t w[16];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) {
-                        f32x2 y = fma2(pack2u(x[g][2 * u], x[g][2 * u + 1]), cc, rr2);
+                        f32x2 y = fma2(pack2u(x[g & 1][2 * u], x[g & 1][2 * u + 1]), cc, rr2);
                         float a, d;
-                        if (u % 4 == 3) {
+                        if (u % kPpPoly == kPpPoly - 1) {
                             y = ex2_poly(y);
                             unpack2(y, a, d);
                         } else {
@@ -568,10 +591,12 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                         w[u] = f32x2_to_bf16(a, d);
                     }
                     tmem_st16(sc + 16 * g, w);                   // over scores that have been read
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar((g == 0 ? PB_P : PB_P2) + t));
+                    if ((g + 1) % (NG / 2) == 0) {               // half of the positions: their products can begin
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar((g + 1 == NG / 2 ? PB_P : PB_P2) + t));
+                    }
                 }
                 float sa, sb, sd, se;
                 unpack2(sum[0], sa, sb);
@@ -583,15 +608,17 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 good = good && __all_sync(0xffffffffu, wait(PB_O + t, 0));
                 tc_fence_after();
             }
-            pair_sync();                                         // the maxima have been read
-            shared_row[t][half][r] = l;
-            pair_sync();
-            l = shared_row[t][0][r] + shared_row[t][1][r];       // the same sum in both threads
+            if constexpr (HALVES == 2) {
+                pair_sync();                                     // the maxima have been read
+                shared_row[t][half][r] = l;
+                pair_sync();
+                l = shared_row[t][0][r] + shared_row[t][1][r];   // the same sum in both threads
+            }
             const float inv = pos < 0 ? 0.f : p.c.v_scale * (Q4 ? kPpCodeScale : 1.f) / l;
             bool odd = false;
             if (good) {
 #pragma unroll 1
-                for (int e = half * (HD / 64); e < (half + 1) * (HD / 64); ++e) {
+                for (int e = half * (HD / 32 / HALVES); e < (half + 1) * (HD / 32 / HALVES); ++e) {
                     uint32_t o[32];
                     if (steps > 0) {
                         tmem_ld32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
@@ -642,7 +669,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             if (lane == 0) odd_rows[t][half][warp & 3] = mine;
             pair_sync();                                         // (what either warp has written is written)
             if (half == 0) {
-                for (unsigned again = odd_rows[t][0][warp & 3] | odd_rows[t][1][warp & 3]; again; again &= again - 1) {
+                for (unsigned again = odd_rows[t][0][warp & 3] | odd_rows[t][HALVES - 1][warp & 3]; again; again &= again - 1) {
                     const int src = __ffs(again) - 1;
                     careful_row<KVT, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
                 }
