@@ -470,6 +470,7 @@ extern "C" int mlb_op_attn_paged(mlb_ops* o, const mlb_paged_kv* kv, const mlb_n
     p.r = rows_of(o, rows);
     p.q = q; p.q_stride = q_stride; p.gate = gate_or_null; p.out = out; p.out_stride = out_stride;
     p.heads = heads; p.group = heads / kv->kv_heads;
+    p.group_inv = p.group > 1 ? (uint32_t)((1ull << 32) / (uint32_t)p.group + 1) : 0;
     p.scale = scale != 0.f ? scale : 1.f / std::sqrt((float)kv->head_dim);
     p.window = std::min(window, 1 << 30);        // no position reaches that far (pt_stride), and differences stay within 32 bits
     p.sinks = std::min(sinks, 1 << 30);

@@ -36,6 +36,7 @@ struct PagedSeq {
 
 __device__ __forceinline__ PagedSeq paged_seq(const PagedRows& p, int pt_stride, int b, bool report) {
     PagedSeq s;
+    s.len = max(0, p.kv_lens[b]);                // (on its way together with the others)
     if (p.row_start) {
         s.r0 = p.row_start[b];
         const int r1 = p.row_start[b + 1];
@@ -51,7 +52,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedRows& p, int pt_stride,
         s.r0 = b;
         s.n = b < p.rows ? 1 : 0;
     }
-    s.len = max(0, p.kv_lens[b]);
     if (s.n > 0 && s.len > (long long)pt_stride * kKvBlock) {
         if (report) atomicExch(p.err, PG_LONG);
         s.n = 0;
@@ -138,6 +138,7 @@ struct AttnPagedParams {
     const float* gate;
     void* out; long long out_stride;
     int heads, group;           // query heads, and per K/V head
+    uint32_t group_inv;         // 2^32 / group + 1, of more than one
     float scale;                // of the scores
     int window, sinks;
     float* part;                // partial results, paged_part_floats() each
@@ -163,6 +164,8 @@ __device__ __forceinline__ PagedSpan paged_span(const AttnPagedParams& p, int pa
     s.count = s.sink_pages + pb / kKvBlock - s.first + 1;
     return s;
 }
+// x / group by a product: exact for x < 2^32 / group, and a call's rows times group are under 2^28
+__device__ __forceinline__ int per_group(const AttnPagedParams& p, int x) { return p.group > 1 ? (int)__umulhi((uint32_t)x, p.group_inv) : x; }
 __device__ __forceinline__ bool paged_sees(const AttnPagedParams& p, int pos, int key) {
     return key <= pos && (p.window <= 0 || key > pos - p.window || key < p.sinks);
 }

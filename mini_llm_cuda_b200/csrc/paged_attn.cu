@@ -622,6 +622,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __gri
     k.b = b;
     k.s = paged_seq(p.r, p.c.pt_stride, b, false);
     const int blocks = split_blocks(p, k.s.n);
+    pdl_launch_dependents();
     pdl_wait();
     if (item >= blocks * p.c.kv_heads) return;
     k.kvh = item / blocks;
@@ -780,20 +781,6 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     if (__any_sync(0xffffffffu, odd)) careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
 }
 
-template <typename... KArgs>
-cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t st, KArgs... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename KVT, typename RT, int HD, int TEAM>
 cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
     using S = SplitShape<KVT, RT, HD>;
@@ -806,7 +793,7 @@ cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const int blocks = p.r.row_start ? kSplitRows / 8 : 1;
     const int rows = p.r.row_start ? 8 : std::min(8, p.group);
-    return launch_after(attn_join_kernel<KVT, RT, HD, TEAM>, dim3(p.r.batch * p.c.kv_heads * blocks, TEAM == 1 ? 1 : rows), 32 * kSplitWarps, st, p, blocks);
+    return launch_after(attn_join_kernel<KVT, RT, HD, TEAM>, dim3(p.r.batch * p.c.kv_heads * blocks, TEAM == 1 ? 1 : rows), 32 * kSplitWarps, 0, st, p, blocks);
 }
 
 template <typename KVT, typename RT, int HD>

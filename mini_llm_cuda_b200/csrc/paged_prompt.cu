@@ -234,12 +234,13 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     auto release = [&]() { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * TILES)); };
     if (found[0] < 0) {                          // (uniform)
         if (warp == kIssuer) release();
+        pdl_wait();
         return;
     }
     const int b = found[0], kvh = (int)((gridDim.x - 1 - blockIdx.x) % (unsigned)p.c.kv_heads), first = found[1] * 128 * TILES;
     const PagedSeq s = {found[2], found[3], found[4]};
     const int count = min(128 * TILES, s.n * p.group - first), tiles = TILES == 2 && count > 128 ? 2 : 1;
-    const int pos0 = s.len - s.n, low = pos0 + first / p.group, high = pos0 + (first + count - 1) / p.group;
+    const int pos0 = s.len - s.n, low = pos0 + per_group(p, first), high = pos0 + per_group(p, first + count - 1);
     const PagedSpan span = paged_span(p, low, high);
     const int steps = (span.count + kPpPages - 1) / kPpPages;
     auto wait = [&](int i, uint32_t parity) {
@@ -413,8 +414,8 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         // The warps of a row's two threads, four apart, share its 32 lanes of tensor memory.
         const int t = warp / (4 * HALVES), half = HALVES == 2 ? warp / 4 & 1 : 0, r = tid & 127, i = t * 128 + r;      // this thread's row of the CTA's
         const bool in = i < count;
-        const int rr = first + (in ? i : 0), row = s.r0 + rr / p.group, h = kvh * p.group + rr % p.group;
-        const int pos = in ? pos0 + rr / p.group : high;
+        const int rr = first + (in ? i : 0), tok = per_group(p, rr), row = s.r0 + tok, h = kvh * p.group + rr - tok * p.group;
+        const int pos = in ? pos0 + tok : high;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // the warp's 32 lanes of tensor memory
         const int pair = 1 + t * 4 + (warp & 3);                      // named barrier of the two warps of these rows
         auto pair_sync = [&]() {
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             x.r = (warp & 3) * 32 + half * (32 / HALVES) + k * (32 / CH) + lane / CH;
             x.c = lane % CH;
             x.in = t * 128 + x.r < count;
-            const int a = first + (x.in ? t * 128 + x.r : 0), token = a / p.group;
+            const int a = first + (x.in ? t * 128 + x.r : 0), token = per_group(p, a);
             x.row = s.r0 + token;
             x.col = (long long)(kvh * p.group + a - token * p.group) * HD + x.c * 8;
             return x;
@@ -683,6 +684,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         tc_fence_after();
         release();
     }
+    pdl_wait();                                  // nothing here needs the kernels before, but the next one in the stream may, and it waits for this one alone
 }
 
 template <typename KVT, int HD>
@@ -697,8 +699,8 @@ cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st)
     cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<KVT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles<KVT>) + p.r.batch;
-    attn_prompt_kernel<KVT, HD><<<(unsigned)(tiles * p.c.kv_heads), kPpThreads<KVT>, smem, st>>>(tk, tv, p);
-    return cudaGetLastError();
+    // It starts while the kernels of the short sequences, which it shares nothing with, are at work.
+    return launch_after(attn_prompt_kernel<KVT, HD>, dim3((unsigned)(tiles * p.c.kv_heads)), kPpThreads<KVT>, smem, st, tk, tv, p);
 }
 
 }  // namespace

@@ -73,6 +73,22 @@ static __device__ __noinline__ void careful_row(const AttnPagedParams& p, int b,
     }
 }
 
+// A launch that need not wait for the kernel before it: that one says when (pdl_launch_dependents), and this one waits itself for its end (pdl_wait)
+template <typename... KArgs>
+static cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, KArgs... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Sequences of up to this many (token, head) rows per K/V head are taken page by page (paged_attn.cu), longer ones in tiles.
 constexpr int kSplitRows = 32;
 
