@@ -143,7 +143,7 @@ struct AttnPagedParams {
     int window, sinks;
     float* part;                // partial results, paged_part_floats() each
     unsigned long long* plan;   // [batch + 1] pages before a sequence, as the splitting kernel laid them out
-    int max_teams;
+    int max_teams, item_cost;   // of the splitting kernel
 };
 
 // Pages that a block of rows sees: `sink_pages` from the first one on, then those from `first` on; `count` in all.

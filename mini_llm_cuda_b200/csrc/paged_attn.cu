@@ -301,11 +301,35 @@ __device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Blo
     const bool in = g < k.count;
     const int r = k.first + (in ? g : 0), row = k.s.r0 + r / p.group, h = k.kvh * p.group + r % p.group;
     const RT* q = static_cast<const RT*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD;
+    // four neighbouring dims for each k-step, all on their way at once
+    float x[HD / 16][4];
+    const bool vec = reinterpret_cast<uintptr_t>(q) % (4 * sizeof(RT)) == 0;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+        const RT* src = q + F::dim(ks, j, 0);
+        if (!in) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[ks][e] = 0.f;
+        } else if (!vec) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[ks][e] = Elem<RT>::get(src, e);
+        } else if constexpr (sizeof(RT) == 4) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(src));
+            x[ks][0] = w.x; x[ks][1] = w.y; x[ks][2] = w.z; x[ks][3] = w.w;
+        } else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+            x[ks][0] = __uint_as_float(w.x << 16); x[ks][1] = __uint_as_float(w.x & 0xffff0000u);
+            x[ks][2] = __uint_as_float(w.y << 16); x[ks][3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+    }
     float up = 1.f, down = 1.f;
     if (F16) {
         // a power of two that brings the row's largest magnitude to 256 .. 512, if it is a number
         float top = 0.f;
-        for (int d = j; d < HD; d += 4) top = fmaxf(top, fabsf(Elem<RT>::get(q, d)));
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[ks][e]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = max(-100, min(100, 8 - ((int)(__float_as_uint(top) >> 23) - 127)));
@@ -315,12 +339,9 @@ __device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Blo
     if (j == 0) qscale[g] = p.scale * p.c.k_scale * 1.4426950408889634f * down;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = in ? Elem<RT>::get(q, F::dim(ks, j, e)) * up : 0.f;
         uint32_t lo[QP], hi[QP];
-        pieces<F16, QP>(x[0], x[1], lo);
-        pieces<F16, QP>(x[2], x[3], hi);
+        pieces<F16, QP>(x[ks][0] * up, x[ks][1] * up, lo);
+        pieces<F16, QP>(x[ks][2] * up, x[ks][3] * up, hi);
 #pragma unroll
         for (int i = 0; i < QP; ++i) qf[(i * (HD / 16) + ks) * 32 + lane] = make_uint2(lo[i], hi[i]);
     }
@@ -337,10 +358,22 @@ struct SplitShape {
 };
 __host__ __device__ constexpr int split_part_floats(int hd) { return 8 * (hd + 2); }
 
+// The first of a warp's pages: its id, K on its way, and the id of the next
+template <typename KVT, int HD>
+struct FirstPage {
+    PageFrag<KVT, HD> f;
+    int id = 0, next = 0;
+    __device__ __forceinline__ FirstPage(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step) {
+        if (v >= v1) return;
+        id = paged_page(p.c, p.r.err, k.b, span.page(v), 0);
+        if (v + step < v1) next = paged_page(p.c, p.r.err, k.b, span.page(v + step), 0);
+        f.load_k(p.c, ((size_t)id * p.c.kv_heads + k.kvh) * kKvBlock, (threadIdx.x & 31) >> 2, threadIdx.x & 3);
+    }
+};
 // The pages v, v + step, .. < v1 of a span for a block; results in acc, m (log2 of the reference of the weights) and l
 template <typename KVT, typename RT, int HD>
-__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, const uint2* qf,
-                                           const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
+__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, FirstPage<KVT, HD>& at,
+                                           const uint2* qf, const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
     using S = SplitShape<KVT, RT, HD>;
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
 #pragma unroll
@@ -357,10 +390,8 @@ __device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block
     const int low = pos0 + k.first / p.group, high = pos0 + (k.first + k.count - 1) / p.group;      // positions of the block's rows
     const float c0 = qscale[2 * j], c1 = qscale[2 * j + 1];
     auto base_of = [&](int id) { return ((size_t)id * p.c.kv_heads + k.kvh) * kKvBlock; };
-    PageFrag<KVT, HD> f;
-    int id = paged_page(p.c, p.r.err, k.b, span.page(v), 0);
-    f.load_k(p.c, base_of(id), g, j);
-    int next = v + step < v1 ? paged_page(p.c, p.r.err, k.b, span.page(v + step), 0) : 0;
+    PageFrag<KVT, HD>& f = at.f;
+    int id = at.id, next = at.next;
 #pragma unroll 1
     for (; v < v1; v += step) {
         const int key0 = span.page(v) * kKvBlock;
@@ -448,13 +479,25 @@ __device__ __forceinline__ int split_blocks(const AttnPagedParams& p, int n) {
     return rows > kSplitRows ? 0 : (int)((rows + 7) / 8);
 }
 
-__device__ __forceinline__ unsigned long long share_start(unsigned long long total, int teams, int t) {
-    return total / (unsigned)teams * (unsigned)t + total % (unsigned)teams * (unsigned)t / (unsigned)teams;
-}
-__device__ __forceinline__ int split_teams(unsigned long long total, int max_teams, int min_pages) {
-    const unsigned long long n = total / (unsigned)min_pages;
-    return n < 1 ? 1 : n < (unsigned)max_teams ? (int)n : max_teams;
-}
+// The total cut into equal shares, the first `more` of them one larger
+struct Shares {
+    unsigned long long each;
+    unsigned teams, more;
+    __device__ __forceinline__ static unsigned long long div(unsigned long long a, unsigned long long b) {
+        return (a | b) >> 32 ? a / b : (unsigned)a / (unsigned)b;
+    }
+    __device__ __forceinline__ Shares(unsigned long long total, int max_teams, int least) {
+        const unsigned long long n = div(total, (unsigned)least);
+        teams = n < 1 ? 1u : n < (unsigned)max_teams ? (unsigned)n : (unsigned)max_teams;
+        each = div(total, teams);
+        more = (unsigned)(total - each * teams);
+    }
+    __device__ __forceinline__ unsigned long long start(unsigned t) const { return each * t + min(t, more); }
+    __device__ __forceinline__ unsigned holder(unsigned long long x) const {         // of x < total
+        const unsigned long long big = (each + 1) * more;
+        return x < big ? (unsigned)div(x, each + 1) : more + (unsigned)div(x - big, each);
+    }
+};
 
 // TEAM: warps of a team, 1 or kSplitWarps
 template <typename KVT, typename RT, int HD, int TEAM>
@@ -476,7 +519,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         if (b < p.r.batch) {
             const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0);
             const int blocks = split_blocks(p, s.n);
-            if (blocks > 0) n = (unsigned long long)max(1, paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
+            if (blocks > 0) n = (unsigned long long)max(1, p.item_cost + paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
         }
         unsigned long long x = n;
 #pragma unroll
@@ -502,10 +545,10 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         for (int b = tid; b <= p.r.batch; b += 32 * kSplitWarps) p.plan[b] = plan[b];
     const unsigned long long total = before;
     if (total == 0) return;
-    const int teams = split_teams(total, p.max_teams, 2 * TEAM);
-    const int team = TEAM == 1 ? (int)blockIdx.x * kSplitWarps + warp : (int)blockIdx.x;
-    if (team >= teams) return;
-    const unsigned long long start = share_start(total, teams, team), end = share_start(total, teams, team + 1);
+    const Shares shares(total, p.max_teams, TEAM + p.item_cost);
+    const unsigned team = TEAM == 1 ? blockIdx.x * kSplitWarps + warp : blockIdx.x;
+    if (team >= shares.teams) return;
+    const unsigned long long start = shares.start(team), end = shares.start(team + 1);
     int b = 0, hi = p.r.batch;
     while (hi - b > 1) {
         const int mid = (b + hi) / 2;
@@ -521,20 +564,21 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         k.s = paged_seq(p.r, p.c.pt_stride, b, false);
         const int blocks = split_blocks(p, k.s.n);
         const PagedSpan span = paged_span(p, k.s.len - k.s.n, k.s.len - 1);
-        const int count = max(1, span.count);
-        const unsigned rest = (unsigned)(at - plan[b]), item = rest / (unsigned)count;
-        const int v0 = (int)(rest % (unsigned)count);
-        const unsigned long long left = end - at;
-        const int v1 = left < (unsigned long long)(count - v0) ? v0 + (int)left : count;
-        k.kvh = (int)item / blocks;
-        k.first = (int)item % blocks * 8;
+        const unsigned count = (unsigned)max(1, span.count + p.item_cost);
+        const unsigned long long rest = at - plan[b], left = end - at, item64 = Shares::div(rest, count);
+        const unsigned c0 = (unsigned)(rest - item64 * count), c1 = left < count - c0 ? c0 + (unsigned)left : count, item = (unsigned)item64;
+        const int v0 = max(0, (int)c0 - p.item_cost), v1 = max(0, (int)c1 - p.item_cost);      // pages
+        k.kvh = (int)(item / (unsigned)blocks);
+        k.first = (int)(item % (unsigned)blocks) * 8;
         k.count = min(8, k.s.n * p.group - k.first);
+        const int mine0 = v0 + (TEAM > 1 ? warp : 0);
+        FirstPage<KVT, HD> page(p, k, span, mine0, min(v1, span.count), TEAM);
         __syncwarp();
         pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
         __syncwarp();
         float acc[HD / 16][4], m[2], l[2];
-        walk_pages<KVT, RT, HD>(p, k, span, v0 + (TEAM > 1 ? warp : 0), min(v1, span.count), TEAM, qf, qscale, acc, m, l);
-        const bool whole = v0 == 0 && v1 == count;
+        walk_pages<KVT, RT, HD>(p, k, span, mine0, min(v1, span.count), TEAM, page, qf, qscale, acc, m, l);
+        const bool whole = c0 == 0 && c1 == count;
         float* part = p.part + ((size_t)team * 2 + (at == start ? 0 : 1)) * S::PART;
         if constexpr (TEAM == 1) {
             bool odd = false;
@@ -605,7 +649,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
             }
             __syncthreads();
         }
-        at += (unsigned)(v1 - v0);
+        at += c1 - c0;
     }
 }
 
@@ -615,70 +659,113 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __gri
     using S = SplitShape<KVT, RT, HD>;
     constexpr int WPR = TEAM == 1 ? 1 : kSplitWarps;
     __shared__ float red[kSplitWarps][HD + 2];
+    __shared__ unsigned long long sums[2][kSplitWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = max_blocks * p.c.kv_heads, b = (int)blockIdx.x / per, item = (int)blockIdx.x % per;
     const int i = WPR == 1 ? warp : (int)blockIdx.y;
+    pdl_launch_dependents();
+    // Where the item lies in the plan, while the other kernel is at work: worked out again where a thread has one sequence at most, else read
+    unsigned long long total = 0, o0 = 0;
+    const bool own_plan = p.r.batch <= 32 * kSplitWarps;
+    if (own_plan) {
+        unsigned long long n = 0;
+        if ((int)threadIdx.x < p.r.batch) {
+            const PagedSeq s = paged_seq(p.r, p.c.pt_stride, threadIdx.x, false);
+            const int blocks = split_blocks(p, s.n);
+            if (blocks > 0) n = (unsigned long long)max(1, p.item_cost + paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
+        }
+        unsigned long long before = (int)threadIdx.x < b ? n : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        if (lane == 0) { sums[0][warp] = n; sums[1][warp] = before; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; ++w) { total += sums[0][w]; o0 += sums[1][w]; }
+    }
     Block k;
     k.b = b;
     k.s = paged_seq(p.r, p.c.pt_stride, b, false);
     const int blocks = split_blocks(p, k.s.n);
-    pdl_launch_dependents();
-    pdl_wait();
-    if (item >= blocks * p.c.kv_heads) return;
-    k.kvh = item / blocks;
-    k.first = item % blocks * 8;
-    k.count = min(8, k.s.n * p.group - k.first);
-    if (i >= k.count) return;
-    const int count = max(1, paged_span(p, k.s.len - k.s.n, k.s.len - 1).count);
-    const unsigned long long total = __ldcg(p.plan + p.r.batch), o0 = __ldcg(p.plan + b) + (unsigned long long)item * count, o1 = o0 + count;
-    const int teams = split_teams(total, p.max_teams, 2 * TEAM);
-    // the team that holds page x: the last one that starts at or before it, x * teams / total or the next one
-    auto holder = [&](unsigned long long x) {
-        int t = (int)(x * (unsigned)teams / total);
-        while (t + 1 < teams && share_start(total, teams, t + 1) <= x) ++t;
-        return t;
-    };
-    const int t0 = holder(o0), t1 = holder(o1 - 1);
+    if (!own_plan) {
+        pdl_wait();
+        total = __ldcg(p.plan + p.r.batch);
+        o0 = __ldcg(p.plan + b);
+    }
+    const bool mine = item < blocks * p.c.kv_heads;
+    k.kvh = mine ? item / blocks : 0;
+    k.first = mine ? item % blocks * 8 : 0;
+    k.count = mine ? min(8, k.s.n * p.group - k.first) : 0;
+    if (i >= k.count) {
+        if (own_plan) pdl_wait();
+        return;
+    }
+    const unsigned count = (unsigned)max(1, paged_span(p, k.s.len - k.s.n, k.s.len - 1).count + p.item_cost);
+    o0 += (unsigned long long)item * count;
+    const Shares shares(total, p.max_teams, TEAM + p.item_cost);
+    const unsigned t0 = shares.holder(o0), t1 = shares.holder(o0 + count - 1), slot0 = shares.start(t0) == o0 ? 0 : 1;
+    if (own_plan) pdl_wait();
     if (t0 == t1) return;                        // one team held it all and wrote the result
-    const int slot0 = share_start(total, teams, t0) == o0 ? 0 : 1;
-    auto part_of = [&](int t) { return p.part + ((size_t)t * 2 + (t == t0 ? slot0 : 0)) * S::PART + i * S::W; };
-    float mx = -INFINITY;
-    for (int t = t0 + lane; t <= t1; t += 32) mx = fmaxf(mx, __ldcg(part_of(t) + HD));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float ref = mx == -INFINITY ? 0.f : mx;
+    // partial results, four at a time: maximum so far, total and sums
+    float mx = -INFINITY, lt = 0.f;
     float2 o[HD / 64];
-    float lt = 0.f;
 #pragma unroll
     for (int e = 0; e < HD / 64; ++e) o[e] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int t = t0 + (WPR == 1 ? 0 : warp); t <= t1; t += WPR) {
-        const float* r = part_of(t);
-        const float f = ex2(__ldcg(r + HD) - ref);
-        lt = fmaf(__ldcg(r + HD + 1), f, lt);
+    for (unsigned t = t0 + (WPR == 1 ? 0 : warp); t <= t1; t += 4 * WPR) {
+        float pm[4], pl[4];
+        float2 x[4][HD / 64];
 #pragma unroll
-        for (int e = 0; e < HD / 64; ++e) {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(r + e * 64 + lane * 2));
-            o[e].x = fmaf(x.x, f, o[e].x);
-            o[e].y = fmaf(x.y, f, o[e].y);
+        for (int u = 0; u < 4; ++u) {
+            const unsigned tu = t + u * WPR;
+            pm[u] = -INFINITY;
+            pl[u] = 0.f;
+            const float* r = p.part + ((size_t)tu * 2 + (tu == t0 ? slot0 : 0)) * S::PART + i * S::W;
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) x[u][e] = tu <= t1 ? __ldcg(reinterpret_cast<const float2*>(r + e * 64 + lane * 2)) : make_float2(0.f, 0.f);
+            if (tu <= t1) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(r + HD));
+                pm[u] = ml.x;
+                pl[u] = ml.y;
+            }
+        }
+        const float mn = fmaxf(fmaxf(mx, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3])), ref = mn == -INFINITY ? 0.f : mn, f = ex2(mx - ref);
+        mx = mn;
+        lt *= f;
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) { o[e].x *= f; o[e].y *= f; }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float fu = ex2(pm[u] - ref);
+            lt = fmaf(pl[u], fu, lt);
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) {
+                o[e].x = fmaf(x[u][e].x, fu, o[e].x);
+                o[e].y = fmaf(x[u][e].y, fu, o[e].y);
+            }
         }
     }
     if constexpr (WPR > 1) {
 #pragma unroll
         for (int e = 0; e < HD / 64; ++e) *reinterpret_cast<float2*>(&red[warp][e * 64 + lane * 2]) = o[e];
-        if (lane == 0) red[warp][HD] = lt;
+        if (lane == 0) { red[warp][HD] = mx; red[warp][HD + 1] = lt; }
         __syncthreads();
         if (warp > 0) return;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) mx = fmaxf(mx, red[w][HD]);
+        const float ref = mx == -INFINITY ? 0.f : mx;
         lt = 0.f;
 #pragma unroll
         for (int e = 0; e < HD / 64; ++e) o[e] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WPR; ++w) {
-            lt += red[w][HD];
+            const float f = ex2(red[w][HD] - ref);
+            lt = fmaf(red[w][HD + 1], f, lt);
 #pragma unroll
             for (int e = 0; e < HD / 64; ++e) {
-                o[e].x += red[w][e * 64 + lane * 2];
-                o[e].y += red[w][e * 64 + lane * 2 + 1];
+                o[e].x = fmaf(red[w][e * 64 + lane * 2], f, o[e].x);
+                o[e].y = fmaf(red[w][e * 64 + lane * 2 + 1], f, o[e].y);
             }
         }
     }
@@ -739,10 +826,11 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     k.count = min(8, k.s.n * p.group - k.first);
     const int pos0 = k.s.len - k.s.n;
     const PagedSpan span = paged_span(p, pos0 + k.first / p.group, pos0 + (k.first + k.count - 1) / p.group);
+    FirstPage<KVT, HD> page(p, k, span, warp, span.count, kSplitWarps);
     if (warp == 0) pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, qf, qscale, lane);
     __syncthreads();
     float acc[HD / 16][4], m[2], l[2];
-    walk_pages<KVT, RT, HD>(p, k, span, warp, span.count, kSplitWarps, qf, qscale, acc, m, l);
+    walk_pages<KVT, RT, HD>(p, k, span, warp, span.count, kSplitWarps, page, qf, qscale, acc, m, l);
     float* mine = red + warp * S::PART;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -789,6 +877,9 @@ cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int ctas = 2 * sm_count;
     p.max_teams = TEAM == 1 ? ctas * kSplitWarps : ctas;
+    // Beside its pages an item costs what comes before and after them, about as much as two pages of each of its team's warps. Where a share has parts of two
+    // items at most, each of its CTA's own, that is the same for all and left out.
+    p.item_cost = (long long)p.r.batch * p.c.kv_heads * 4 >= p.max_teams ? 2 * TEAM : 0;
     attn_split_kernel<KVT, RT, HD, TEAM><<<ctas, 32 * kSplitWarps, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const int blocks = p.r.row_start ? kSplitRows / 8 : 1;
