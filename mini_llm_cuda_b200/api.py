@@ -499,68 +499,82 @@ class Ops:
         L = lib()
         self._append, self._read, self._attn = L.mlb_op_kv_append, L.mlb_op_kv_read, L.mlb_op_attn_paged
 
-    def _rows(self, x, what: str, rows: NewRows, width: int, dtype):
+    def _rows(self, x, what: str, shape: tuple, dtype):
         """(pointer, stride) of a row tensor; called for every tensor of every call, so the common case is checked first."""
-        shape = x.shape
-        if x.dtype is not dtype or x.get_device() != self.device or len(shape) != 2 or shape[0] != rows.rows or shape[1] != width or \
-                (x.stride(1) != 1 and width > 1):
-            if x.dtype is not dtype:
-                raise ValueError(f"{what} is {x.dtype}: expected {dtype}")
-            if x.get_device() != self.device:
-                raise ValueError(f"{what} is not on CUDA device {self.device}")
-            if len(shape) != 3 or shape[0] != rows.rows or shape[1] * shape[2] != width or x.stride(2) != 1 or x.stride(1) != shape[2]:
-                raise ValueError(f"{what} must be [{rows.rows}][{width}], dense within a row")
+        if x.dtype is dtype and x.shape == shape and x.get_device() == self.device:
+            s = x.stride()
+            if s[1] == 1 or shape[1] == 1:
+                return x.data_ptr(), s[0]
+        rows, width = shape
+        if x.dtype is not dtype:
+            raise ValueError(f"{what} is {x.dtype}: expected {dtype}")
+        if x.get_device() != self.device:
+            raise ValueError(f"{what} is not on CUDA device {self.device}")
+        s = x.shape
+        if len(s) != 3 or s[0] != rows or s[1] * s[2] != width or x.stride(2) != 1 or x.stride(1) != s[2]:
+            raise ValueError(f"{what} must be [{rows}][{width}], dense within a row")
         return x.data_ptr(), x.stride(0)
 
     def _check(self, cache: PagedKV, rows: NewRows, x, what: str) -> int:
-        if cache.batch < rows.batch:
-            raise ValueError(f"the page table has {cache.batch} rows, the call {rows.batch} sequences")
-        if cache.device != self.device or rows.device != self.device:
-            raise ValueError(f"the cache and its rows must be on CUDA device {self.device}")
-        dt = _row_dtype(x.dtype)
-        if dt is None:
+        dt = _dtype_seen.get(x.dtype) or _row_dtype(x.dtype)
+        if dt is None or cache.batch < rows.batch or cache.device != self.device or rows.device != self.device:
+            if cache.batch < rows.batch:
+                raise ValueError(f"the page table has {cache.batch} rows, the call {rows.batch} sequences")
+            if dt is not None:
+                raise ValueError(f"the cache and its rows must be on CUDA device {self.device}")
             raise ValueError(f"{what} is {x.dtype}: expected float32 or bfloat16")
         return dt
 
     def kv_append(self, cache: PagedKV, rows: NewRows, k, v, rope=None, q=None, q_out=None, heads: int = 0, stream: int = 0):
         """Rotates k (and q into q_out, which may be q) by the rows' positions and writes k and v to their pages."""
-        dtype = k.dtype
+        dtype, shape = k.dtype, (rows.rows, cache.width)
         dt = self._check(cache, rows, k, "k")
-        kp, ks = self._rows(k, "k", rows, cache.width, dtype)
-        vp_, vs = self._rows(v, "v", rows, cache.width, dtype)
+        kp, ks = self._rows(k, "k", shape, dtype)
+        vp_, vs = self._rows(v, "v", shape, dtype)
         qp, qs, op, os_ = None, 0, None, 0
         if q is not None:
-            qp, qs = self._rows(q, "q", rows, heads * cache.head_dim, dtype)
-            op, os_ = self._rows(q_out, "q_out", rows, heads * cache.head_dim, dtype)
+            shape = (rows.rows, heads * cache.head_dim)
+            qp, qs = self._rows(q, "q", shape, dtype)
+            if q_out is q:
+                op, os_ = qp, qs
+            else:
+                op, os_ = self._rows(q_out, "q_out", shape, dtype)
         rp, rl = None, 0
         if rope is not None:
             shape = rope.shape
-            if _row_dtype(rope.dtype) != DT_F32 or len(shape) != 2 or shape[1] != cache.head_dim or not rope.is_contiguous() or \
-                    rope.get_device() != self.device:
+            if _dtype_seen.get(rope.dtype) != DT_F32 and _row_dtype(rope.dtype) != DT_F32 or len(shape) != 2 or shape[1] != cache.head_dim or \
+                    not rope.is_contiguous() or rope.get_device() != self.device:
                 raise ValueError(f"rope must be a contiguous fp32 [positions][{cache.head_dim}] on CUDA device {self.device}")
             rp, rl = rope.data_ptr(), shape[0]
-        check(self._append(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, rp, rl, qp, qs, op, os_, heads, stream))
+        rc = self._append(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, rp, rl, qp, qs, op, os_, heads, stream)
+        if rc:
+            check(rc)
 
     def kv_read(self, cache: PagedKV, rows: NewRows, k_out, v_out, stream: int = 0):
         """The rows' cached keys and values, as values."""
+        dtype, shape = k_out.dtype, (rows.rows, cache.width)
         dt = self._check(cache, rows, k_out, "k_out")
-        kp, ks = self._rows(k_out, "k_out", rows, cache.width, k_out.dtype)
-        vp_, vs = self._rows(v_out, "v_out", rows, cache.width, k_out.dtype)
-        check(self._read(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, stream))
+        kp, ks = self._rows(k_out, "k_out", shape, dtype)
+        vp_, vs = self._rows(v_out, "v_out", shape, dtype)
+        rc = self._read(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, stream)
+        if rc:
+            check(rc)
 
     def attn_paged(self, cache: PagedKV, rows: NewRows, q, out, heads: int, gate=None, scale: float = 0.0, window: int = 0, sinks: int = 0,
                    stream: int = 0):
         """Causal attention of the rows, optionally within a window and to the first `sinks` positions (mlb_op_attn_paged)."""
+        dtype, shape = q.dtype, (rows.rows, heads * cache.head_dim)
         dt = self._check(cache, rows, q, "q")
-        width = heads * cache.head_dim
-        qp, qs = self._rows(q, "q", rows, width, q.dtype)
-        op, os_ = self._rows(out, "out", rows, width, q.dtype)
+        qp, qs = self._rows(q, "q", shape, dtype)
+        op, os_ = self._rows(out, "out", shape, dtype)
         gp = None
         if gate is not None:
             if _row_dtype(gate.dtype) != DT_F32 or not gate.is_contiguous():
                 raise ValueError("gate must be a contiguous fp32 tensor")
-            gp, _ = self._rows(gate, "gate", rows, width, gate.dtype)
-        check(self._attn(self._h, cache.ref, rows.ref, dt, qp, qs, gp, op, os_, heads, scale, window, sinks, stream))
+            gp, _ = self._rows(gate, "gate", shape, gate.dtype)
+        rc = self._attn(self._h, cache.ref, rows.ref, dt, qp, qs, gp, op, os_, heads, scale, window, sinks, stream)
+        if rc:
+            check(rc)
 
     def status(self, stream: int = 0):
         """Waits for the stream; raises if a call since the last status() met a bad page id, row range or length."""
