@@ -5,6 +5,7 @@
 
 #include "paged_prompt.h"
 #include "paged_row.cuh"
+#include "ring.cuh"
 
 namespace mlb {
 
@@ -35,6 +36,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t to, const void* from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -159,35 +168,48 @@ struct PageFrag<fp4_t, HD> {
     uint32_t k[2][KW], ks_[2], v[4][VW], vs[2];
     __device__ static int dim(int ks, int j, int slot) { return j * (HD / 4) + ks * 4 + slot; }
     __device__ static int vdim(int mt, int g) { return g * (HD / 8) + mt * 2; }
-    __device__ __forceinline__ void load_k(const PagedCache& c, size_t base, int g, int j) {
-        const unsigned char *p = static_cast<const unsigned char*>(c.kpool) + base * (HD / 2), *s = c.kscale + base * (HD / 16);
+    // A page in shared memory: codes of K, of V (of 128 dims, with the 16-byte pieces of a row moved by row / 2, against bank conflicts), scales of K, of V
+    static constexpr int kCodes = 16 * HD / 2, kScales = HD, kBytes = 2 * (kCodes + kScales);
+    __device__ static void copy(const PagedCache& c, size_t base, uint32_t to, int lane) {
+        const unsigned char *k = static_cast<const unsigned char*>(c.kpool) + base * (HD / 2) + lane * 16, *v = static_cast<const unsigned char*>(c.vpool) + base * (HD / 2) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i) {
+            const int piece = lane + 32 * i, row = piece / (HD / 32), ch = piece % (HD / 32);
+            cp_async<16>(to + piece * 16, k + i * 512);
+            cp_async<16>(to + kCodes + row * (HD / 2) + (HD == 128 ? ch ^ (row >> 1 & 3) : ch) * 16, v + i * 512);
+        }
+        if (lane < kScales / 4) {
+            cp_async<4>(to + 2 * kCodes + lane * 4, c.kscale + base * (HD / 16) + lane * 4);
+            cp_async<4>(to + 2 * kCodes + kScales + lane * 4, c.vscale + base * (HD / 16) + lane * 4);
+        }
+    }
+    __device__ __forceinline__ void read_k(const unsigned char* page, int g, int j) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int row = t * 8 + g;
             if constexpr (HD == 128) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + row * 64) + j);
+                const uint4 x = *reinterpret_cast<const uint4*>(page + row * 64 + j * 16);
                 k[t][0] = x.x; k[t][1] = x.y; k[t][2 % KW] = x.z; k[t][3 % KW] = x.w;
-                ks_[t] = __ldg(reinterpret_cast<const unsigned short*>(s + row * 8) + j);
+                ks_[t] = *reinterpret_cast<const unsigned short*>(page + 2 * kCodes + row * 8 + j * 2);
             } else {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(p + row * 32) + j);
+                const uint2 x = *reinterpret_cast<const uint2*>(page + row * 32 + j * 8);
                 k[t][0] = x.x; k[t][1] = x.y;
-                ks_[t] = __ldg(s + row * 4 + j);
+                ks_[t] = page[2 * kCodes + row * 4 + j];
             }
         }
     }
-    __device__ __forceinline__ void load_v(const PagedCache& c, size_t base, int g, int j) {
-        const unsigned char *p = static_cast<const unsigned char*>(c.vpool) + base * (HD / 2), *s = c.vscale + base * (HD / 16);
+    __device__ __forceinline__ void read_v(const unsigned char* page, int g, int j) {
         uint32_t b[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 2 * j + (i & 1) + (i & 2) * 4;
             if constexpr (HD == 128) {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(p + row * 64) + g);
+                const uint2 x = *reinterpret_cast<const uint2*>(page + kCodes + row * 64 + ((g >> 1) ^ j) * 16 + (g & 1) * 8);
                 v[i][0] = x.x; v[i][1 % VW] = x.y;
-                b[i] = __ldg(s + row * 8 + g);
+                b[i] = page[2 * kCodes + kScales + row * 8 + g];
             } else {
-                v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(p + row * 32) + g);
-                b[i] = __ldg(s + row * 4 + g / 2);
+                v[i][0] = *reinterpret_cast<const uint32_t*>(page + kCodes + row * 32 + g * 4);
+                b[i] = page[2 * kCodes + kScales + row * 4 + g / 2];
             }
         }
         vs[0] = b[0] | b[1] << 8;
@@ -264,13 +286,17 @@ __device__ __forceinline__ void page_values(const PageFrag<KVT, HD>& f, const fl
         const uint32_t s0 = e4m3x2_to_f16(f.vs[0]), s1 = e4m3x2_to_f16(f.vs[1]);
 #pragma unroll
         for (int w8 = 0; w8 < F::VW; ++w8) {
+            // codes of one dim and two neighbouring rows side by side, of even dims, of odd ones
             uint32_t h[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e2m1x8_to_f16(f.v[i][w8], h[i]);
+            for (int i = 0; i < 4; i += 2) {
+                const uint32_t x = f.v[i][w8], y = f.v[i + 1][w8];
+                e2m1x8_to_f16((x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u), h[i]);
+                e2m1x8_to_f16((x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), h[i + 1]);
+            }
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const uint32_t a0 = hmul2(__byte_perm(h[0][m], h[1][m], 0x5410), s0), a1 = hmul2(__byte_perm(h[0][m], h[1][m], 0x7632), s0);
-                const uint32_t a2 = hmul2(__byte_perm(h[2][m], h[3][m], 0x5410), s1), a3 = hmul2(__byte_perm(h[2][m], h[3][m], 0x7632), s1);
+                const uint32_t a0 = hmul2(h[0][m], s0), a1 = hmul2(h[1][m], s0), a2 = hmul2(h[2][m], s1), a3 = hmul2(h[3][m], s1);
 #pragma unroll
                 for (int i = 0; i < PP; ++i) mma_f16(acc[w8 * 4 + m], a0, a1, a2, a3, p0[i], p1[i]);
             }
@@ -358,21 +384,91 @@ struct SplitShape {
 };
 __host__ __device__ constexpr int split_part_floats(int hd) { return 8 * (hd + 2); }
 
-// The first of a warp's pages: its id, K on its way, and the id of the next
+// How a warp gets the pages v, v + step, .. < v1: into registers, K of the next one while this one's V is weighed. Made before the queries are
+// packed, so that the first loads are under way.
 template <typename KVT, int HD>
-struct FirstPage {
+struct PageSource {
+    static constexpr int kRing = 0;              // bytes of shared memory
+    const AttnPagedParams& p;
+    const Block& k;
+    const PagedSpan& span;
+    const int v1, step;
     PageFrag<KVT, HD> f;
     int id = 0, next = 0;
-    __device__ __forceinline__ FirstPage(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step) {
+    __device__ __forceinline__ size_t base(int x) const { return ((size_t)x * p.c.kv_heads + k.kvh) * kKvBlock; }
+    __device__ __forceinline__ PageSource(const AttnPagedParams& p_, const Block& k_, const PagedSpan& span_, int v, int v1_, int step_, unsigned char*)
+        : p(p_), k(k_), span(span_), v1(v1_), step(step_) {
         if (v >= v1) return;
         id = paged_page(p.c, p.r.err, k.b, span.page(v), 0);
         if (v + step < v1) next = paged_page(p.c, p.r.err, k.b, span.page(v + step), 0);
-        f.load_k(p.c, ((size_t)id * p.c.kv_heads + k.kvh) * kKvBlock, (threadIdx.x & 31) >> 2, threadIdx.x & 3);
+        f.load_k(p.c, base(id), (threadIdx.x & 31) >> 2, threadIdx.x & 3);
+    }
+    __device__ __forceinline__ void begin(int, int g, int j) { f.load_v(p.c, base(id), g, j); }      // page v
+    __device__ __forceinline__ void k_used(int v, int g, int j) {
+        if (v + step < v1) f.load_k(p.c, base(next), g, j);
+        id = next;
+        if (v + 2 * step < v1) next = paged_page(p.c, p.r.err, k.b, span.page(v + 2 * step), 0);
+    }
+    __device__ __forceinline__ void want_v(int, int) {}
+    __device__ __forceinline__ void end() {}
+};
+// 4-bit pages are small (2.3 KB for 16 positions of K and V, 128 dims): a warp has up to kStages - 1 on their way to a ring in shared memory, and one load
+// brings the ids of 32. (In registers, one page and a half: 2.6 of 7 cycles between a warp's instructions went by waiting for them.)
+template <int HD>
+struct PageSource<fp4_t, HD> {
+    using F = PageFrag<fp4_t, HD>;
+    static constexpr int kStages = 4, kRing = kStages * F::kBytes;
+    const AttnPagedParams& p;
+    const Block& k;
+    const PagedSpan& span;
+    const int v1, step;
+    unsigned char* const ring;
+    F f;
+    int ahead, count = 0, used = 0;              // next page to bring; pages brought, and used
+    int ids = 0, more_ids = 0;                   // of 32 pages, a lane each, and of the 32 after these
+    __device__ __forceinline__ int load_ids(int v) const {
+        v += (int)(threadIdx.x & 31) * step;
+        return v < v1 ? paged_page(p.c, p.r.err, k.b, span.page(v), 0) : 0;
+    }
+    __device__ __forceinline__ void bring() {
+        if (ahead < v1) {
+            const int id = __shfl_sync(0xffffffffu, ids, count & 31);
+            F::copy(p.c, ((size_t)id * p.c.kv_heads + k.kvh) * kKvBlock, smem_u32(ring) + (uint32_t)(count % kStages) * F::kBytes, threadIdx.x & 31);
+            ahead += step;
+            if ((++count & 31) == 0) {
+                ids = more_ids;
+                more_ids = load_ids(ahead + 32 * step);
+            }
+        }
+        cp_async_commit();                       // (an empty group too, so that waits count pages)
+    }
+    __device__ __forceinline__ PageSource(const AttnPagedParams& p_, const Block& k_, const PagedSpan& span_, int v, int v1_, int step_, unsigned char* ring_)
+        : p(p_), k(k_), span(span_), v1(v1_), step(step_), ring(ring_), ahead(v) {
+        ids = load_ids(v);
+        more_ids = load_ids(v + 32 * step);
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) bring();
+    }
+    __device__ __forceinline__ const unsigned char* page() const { return ring + used % kStages * F::kBytes; }
+    __device__ __forceinline__ void begin(int, int g, int j) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();                            // all lanes' pieces are there, and the page before has been used by all
+        bring();
+        f.read_k(page(), g, j);
+    }
+    __device__ __forceinline__ void k_used(int, int, int) {}
+    __device__ __forceinline__ void want_v(int g, int j) {
+        f.read_v(page(), g, j);
+        ++used;
+    }
+    __device__ __forceinline__ void end() {
+        cp_async_wait<0>();
+        __syncwarp();
     }
 };
 // The pages v, v + step, .. < v1 of a span for a block; results in acc, m (log2 of the reference of the weights) and l
 template <typename KVT, typename RT, int HD>
-__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, FirstPage<KVT, HD>& at,
+__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, PageSource<KVT, HD>& src,
                                            const uint2* qf, const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
     using S = SplitShape<KVT, RT, HD>;
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
@@ -382,26 +478,26 @@ __device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block
         for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
-    if (v >= v1) return;
+    if (v >= v1) {
+        src.end();
+        return;
+    }
     const int pos0 = k.s.len - k.s.n;
     int pos[2];
     pos[0] = 2 * j < k.count ? pos0 + (k.first + 2 * j) / p.group : -1;
     pos[1] = 2 * j + 1 < k.count ? pos0 + (k.first + 2 * j + 1) / p.group : -1;
     const int low = pos0 + k.first / p.group, high = pos0 + (k.first + k.count - 1) / p.group;      // positions of the block's rows
     const float c0 = qscale[2 * j], c1 = qscale[2 * j + 1];
-    auto base_of = [&](int id) { return ((size_t)id * p.c.kv_heads + k.kvh) * kKvBlock; };
-    PageFrag<KVT, HD>& f = at.f;
-    int id = at.id, next = at.next;
+    PageFrag<KVT, HD>& f = src.f;
 #pragma unroll 1
     for (; v < v1; v += step) {
         const int key0 = span.page(v) * kKvBlock;
-        f.load_v(p.c, base_of(id), g, j);
+        src.begin(v, g, j);
         float s[4];
         page_scores<KVT, HD, S::QP>(f, qf, lane, s);
-        if (v + step < v1) f.load_k(p.c, base_of(next), g, j);
-        id = next;
-        if (v + 2 * step < v1) next = paged_page(p.c, p.r.err, k.b, span.page(v + 2 * step), 0);
+        src.k_used(v, g, j);
         s[0] *= c0; s[1] *= c1; s[2] *= c0; s[3] *= c1;
+        src.want_v(g, j);
         if (key0 + kKvBlock - 1 > low || (p.window > 0 && key0 <= high - p.window && key0 + kKvBlock > p.sinks)) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -433,11 +529,19 @@ __device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block
         l[1] += s[1] + s[3];
         page_values<KVT, HD, S::PP>(f, s, acc);
     }
+    src.end();
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
         l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
         l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
     }
+}
+
+// Shared memory of a CTA's rings, and of its warps' results, which lie over them
+template <typename KVT, int HD, int TEAM>
+__host__ __device__ constexpr int split_ring_bytes() {
+    constexpr int rings = kSplitWarps * PageSource<KVT, HD>::kRing, results = TEAM > 1 ? kSplitWarps * split_part_floats(HD) * 4 : 0;
+    return rings > results ? rings : results;
 }
 
 // Row i of a block: its row of the call's tensors, head, and position
@@ -505,8 +609,9 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
     using S = SplitShape<KVT, RT, HD>;
     extern __shared__ __align__(16) unsigned char sm[];
     uint2* qf_all = reinterpret_cast<uint2*>(sm);                                        // [warp][QWORDS]
-    float* red = reinterpret_cast<float*>(sm + (size_t)kSplitWarps * S::QWORDS * 8);     // TEAM > 1: [warp][8][W], a row's maximum and total behind its sums
-    unsigned long long* plan = reinterpret_cast<unsigned long long*>(red + (TEAM > 1 ? kSplitWarps * S::PART : 0));      // [batch + 1]
+    unsigned char* ring = sm + (size_t)kSplitWarps * S::QWORDS * 8;
+    float* red = reinterpret_cast<float*>(ring);                                         // TEAM > 1: [warp][8][W], a row's maximum and total behind its sums
+    unsigned long long* plan = reinterpret_cast<unsigned long long*>(ring + split_ring_bytes<KVT, HD, TEAM>());      // [batch + 1]
     __shared__ float qs_all[kSplitWarps][8];
     __shared__ unsigned long long warp_sum_[kSplitWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
@@ -572,7 +677,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         k.first = (int)(item % (unsigned)blocks) * 8;
         k.count = min(8, k.s.n * p.group - k.first);
         const int mine0 = v0 + (TEAM > 1 ? warp : 0);
-        FirstPage<KVT, HD> page(p, k, span, mine0, min(v1, span.count), TEAM);
+        PageSource<KVT, HD> page(p, k, span, mine0, min(v1, span.count), TEAM, ring + warp * PageSource<KVT, HD>::kRing);
         __syncwarp();
         pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
         __syncwarp();
@@ -605,6 +710,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
                 }
             }
         } else {
+            if (PageSource<KVT, HD>::kRing > 0) __syncthreads();         // the rings have been read
             float* mine = red + warp * S::PART;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -783,7 +889,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     using S = SplitShape<KVT, RT, HD>;
     extern __shared__ __align__(16) unsigned char sm[];
     uint2* qf = reinterpret_cast<uint2*>(sm);
-    float* red = reinterpret_cast<float*>(sm + (size_t)S::QWORDS * 8);
+    unsigned char* ring = sm + (size_t)S::QWORDS * 8;
+    float* red = reinterpret_cast<float*>(ring);
     __shared__ float qscale[8];
     __shared__ int found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
@@ -826,11 +933,12 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     k.count = min(8, k.s.n * p.group - k.first);
     const int pos0 = k.s.len - k.s.n;
     const PagedSpan span = paged_span(p, pos0 + k.first / p.group, pos0 + (k.first + k.count - 1) / p.group);
-    FirstPage<KVT, HD> page(p, k, span, warp, span.count, kSplitWarps);
+    PageSource<KVT, HD> page(p, k, span, warp, span.count, kSplitWarps, ring + warp * PageSource<KVT, HD>::kRing);
     if (warp == 0) pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, qf, qscale, lane);
     __syncthreads();
     float acc[HD / 16][4], m[2], l[2];
     walk_pages<KVT, RT, HD>(p, k, span, warp, span.count, kSplitWarps, page, qf, qscale, acc, m, l);
+    if (PageSource<KVT, HD>::kRing > 0) __syncthreads();                 // the rings have been read
     float* mine = red + warp * S::PART;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -872,7 +980,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
 template <typename KVT, typename RT, int HD, int TEAM>
 cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
     using S = SplitShape<KVT, RT, HD>;
-    const size_t smem = (size_t)kSplitWarps * S::QWORDS * 8 + (TEAM > 1 ? (size_t)kSplitWarps * S::PART * 4 : 0) + ((size_t)p.r.batch + 1) * 8;
+    const size_t smem = (size_t)kSplitWarps * S::QWORDS * 8 + split_ring_bytes<KVT, HD, TEAM>() + ((size_t)p.r.batch + 1) * 8;
     cudaError_t e = cudaFuncSetAttribute(attn_split_kernel<KVT, RT, HD, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e != cudaSuccess) return e;
     const int ctas = 2 * sm_count;
@@ -897,7 +1005,7 @@ cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) 
     const long long most = p.r.max_rows > 0 ? std::min(p.r.max_rows, p.r.rows) : p.r.rows;
     if (most * p.group <= kSplitRows) return e;
     if constexpr (sizeof(KVT) <= 2 && sizeof(RT) == 2) return attn_prompt_launch(p, sizeof(KVT) == 1 ? MLB_DT_FP4_E2M1 : MLB_DT_BF16, HD, st);
-    const size_t smem = (size_t)S::QWORDS * 8 + (size_t)kSplitWarps * S::PART * 4;
+    const size_t smem = (size_t)S::QWORDS * 8 + split_ring_bytes<KVT, HD, kSplitWarps>();
     e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e != cudaSuccess) return e;
     const long long blocks = (long long)p.r.rows * p.group / 8 + p.r.batch;
