@@ -29,7 +29,7 @@ template <typename KVT> constexpr int kPpLoaders = sizeof(KVT) == 1 ? 4 : 1;    
 // the tile's products, and 8 such warps on an SM did not hide them. One with 4-bit pages, whose loaders and softmax share the issue slots that bound them.
 template <typename KVT> constexpr int kPpHalves = sizeof(KVT) == 1 ? 1 : 2;
 template <typename KVT> constexpr int kPpThreads = 128 * kPpHalves<KVT> * kPpTiles<KVT> + 32 * kPpLoaders<KVT> + 32;          // softmax warps, loaders, the issuer's
-constexpr int kPpPoly = 4;                       // one pair of so many exponentials by polynomial
+constexpr int kPpPoly = 8;                       // one pair of so many exponentials by polynomial (2: 4 % slower, 4: 2 %, none: none to 2 %)
 constexpr float kPpLazy = 8.f;
 constexpr uint32_t kPpSpin = 1u << 24;
 
@@ -142,13 +142,16 @@ __device__ __forceinline__ void commit_elected(uint32_t mbar) {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <int HD, int TILES>
+// Heads of 64 dims leave room in tensor memory for weights beside the scores, so that the next step's scores are computed as soon as the
+// softmax has this step's in its registers, under its exponentials. (A step of one tile took 3500 cycles, 1900 of them the softmax.)
+template <typename KVT, int HD> constexpr bool kPpEarly = HD == 64 && kPpHalves<KVT> == 2;
+template <int HD, int TILES, bool EARLY>
 struct PromptSmem {
-    static constexpr int stages = TILES;         // of K and V: with one, the other CTA of the SM fills the wait
+    static constexpr int stages = EARLY ? 2 : TILES;      // of K and V: with one, the other CTA of the SM fills the wait
     static constexpr uint32_t kQ = 128 * HD * 2, kKV = kPpKeys * HD * 2, kHalf = 128 * 128;      // bytes of a tile; of 64 dims of one
     static constexpr uint32_t q = 0, k = TILES * kQ, v = k + stages * kKV, bars = v + stages * kKV, total = bars + 256;
 };
-enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_END = 17, PB_COUNT = 18 };
+enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_END = 17, PB_READ = 18, PB_COUNT = 19 };
 
 // 4-bit pages: eight codes (dims 0 .. 7) -> four bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code * scale / 256. Exponent and mantissa of
 // a code are put at the low end of a bf16's exponent, which makes it code * 2^-126 exactly (0.5 as a subnormal), and multiplied by `s`, the
@@ -170,7 +173,9 @@ template <typename KVT, int HD>
 __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     attn_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnPagedParams p) {
     constexpr int TILES = kPpTiles<KVT>;
-    using L = PromptSmem<HD, TILES>;
+    constexpr bool EARLY = kPpEarly<KVT, HD>;
+    using L = PromptSmem<HD, TILES, EARLY>;
+    static_assert(!EARLY || TILES == 1, "columns of tensor memory");
     constexpr int NST = L::stages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -223,14 +228,15 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             found[1] = want;
             for (int i = 0; i < PB_COUNT; ++i) {
                 const bool filled = i == PB_KFULL || i == PB_KFULL + 1 || i == PB_VFULL || i == PB_VFULL + 1;
-                mbar_init(bar(i), i == PB_Q ? 4 * HALVES * TILES : i >= PB_P && i < PB_O ? 4 * HALVES : Q4 && filled ? 128 : 1);
+                mbar_init(bar(i), i == PB_Q ? 4 * HALVES * TILES : (i >= PB_P && i < PB_O) || i == PB_READ ? 4 * HALVES : Q4 && filled ? 128 : 1);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);             // S of each tile, then O of each, 128 columns apart
+    // Columns: S of each tile, then O of each, 128 apart, weights over their scores; or S, weights, O
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0), tmem_p = tmem + (EARLY ? 128 : 0), tmem_o = tmem + (EARLY ? 192 : TILES * 128);
     auto release = [&]() { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * TILES)); };
     if (found[0] < 0) {                          // (uniform)
         if (warp == kIssuer) release();
@@ -374,6 +380,13 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             }
             for (int j = 0; j < steps && good; ++j) {
                 const uint32_t ph = (uint32_t)(j / NST) & 1u;
+                if (EARLY && j + 1 < steps) {
+                    good = all_wait(PB_READ, (uint32_t)j & 1u) && all_wait(PB_KFULL + (j + 1) % NST, (uint32_t)((j + 1) / NST) & 1u);
+                    if (!good) break;
+                    tc_fence_after();
+                    scores(0, j + 1);
+                    commit_elected(bar(PB_KEMPTY + (j + 1) % NST));
+                }
                 for (int t = 0; t < tiles && good; ++t) {
                     good = all_wait(PB_P + t, (uint32_t)j & 1u) && (t > 0 || all_wait(PB_VFULL + j % NST, ph));
                     if (!good) break;
@@ -387,12 +400,13 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                             if (!good) break;
                             tc_fence_after();
                         }
-                        umma_ts(tmem + (TILES + t) * 128, tmem + t * 128 + (HALVES == 2 ? ks / 4 * 64 + ks % 4 * 8 : ks * 8), umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
+                        umma_ts(tmem_o + t * 128, tmem_p + t * 128 + (HALVES == 2 && !EARLY ? ks / 4 * 64 + ks % 4 * 8 : ks * 8), umma_desc_rows_are_k(sm0 + L::v + j % NST * L::kKV + ks * 2048, L::kHalf), io,
                                      j > 0 || i > 0);
                     }
                     if (!good) break;
                     if (t == tiles - 1) commit_elected(bar(PB_VEMPTY + j % NST));
                     if (j + 1 < steps) {
+                        if (EARLY) continue;
                         if (t == 0) {
                             good = all_wait(PB_KFULL + (j + 1) % NST, (uint32_t)((j + 1) / NST) & 1u);
                             if (!good) break;
@@ -532,15 +546,26 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                     if (HALVES == 1 && g + 1 < NG) tmem_ld32(sc + 32 * (g + 1), x[(g + 1) & 1]);
                     if (edge) hide(x[g & 1], g);
                 };
+                if constexpr (EARLY) {                           // (both halves of the scores are waited for together)
+                    arrived(0);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(PB_READ));
+                }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    arrived(g);
+                    if (!EARLY || g > 0) arrived(g);
 #pragma unroll
                     for (int u = 0; u < 32; u += 2)
                         top[u / 2 & 3] = max3_nan(top[u / 2 & 3], __uint_as_float(x[g & 1][u]), __uint_as_float(x[g & 1][u + 1]));
                 }
                 float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], -INFINITY) * c;
+                // the products with the step before's weights are done: O and the weights' columns are this step's
+                if (EARLY && j > 0) {
+                    good = good && __all_sync(0xffffffffu, wait(PB_VEMPTY + (j - 1) % NST, (uint32_t)((j - 1) / NST) & 1u));
+                    tc_fence_after();
+                }
                 // (a score that is no number makes the maximum, and so the row, none)
                 if (pair_any(!(mx <= m + kPpLazy))) {
                     if constexpr (HALVES == 2) {
@@ -556,7 +581,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
 #pragma unroll 1
                         for (int e = half * (HD / 16 / HALVES); e < (half + 1) * (HD / 16 / HALVES); ++e) {
                             uint32_t o[16];
-                            const uint32_t at = tmem + lanes + (TILES + t) * 128 + e * 16;
+                            const uint32_t at = tmem_o + lanes + t * 128 + e * 16;
                             tmem_ld16(at, o);
                             tmem_ld_wait();
                             tmem_loaded(o);
@@ -573,7 +598,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     if (HALVES == 1) arrived(g);
-                    // weights of 32 positions, one pair of four by polynomial: the exponential's unit takes 16 a cycle and would be the bound
+                    // weights of 32 positions, some by polynomial: the exponential's unit takes 16 a cycle
                     uint32_t w[16];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) {
@@ -591,7 +616,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                         sum[u & 1] = add2(sum[u & 1], y);
                         w[u] = f32x2_to_bf16(a, d);
                     }
-                    tmem_st16(sc + 16 * g, w);                   // over scores that have been read
+                    tmem_st16(EARLY ? tmem_p + lanes + half * 32 + 16 * g : sc + 16 * g, w);      // (over scores that have been read)
                     if ((g + 1) % (NG / 2) == 0) {               // half of the positions: their products can begin
                         tmem_st_wait();
                         tc_fence_before();
@@ -622,7 +647,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 for (int e = half * (HD / 32 / HALVES); e < (half + 1) * (HD / 32 / HALVES); ++e) {
                     uint32_t o[32];
                     if (steps > 0) {
-                        tmem_ld32(tmem + lanes + (TILES + t) * 128 + e * 32, o);
+                        tmem_ld32(tmem_o + lanes + t * 128 + e * 32, o);
                         tmem_ld_wait();
                         tmem_loaded(o);
                     }
@@ -695,7 +720,7 @@ cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st)
     const uint64_t rows = (uint64_t)p.c.num_pages * p.c.kv_heads * kKvBlock;
     if (sizeof(KVT) == 2 && (make_bf16_map(enc, &tk, p.c.kpool, rows, HD, kKvBlock) || make_bf16_map(enc, &tv, p.c.vpool, rows, HD, kKvBlock)))
         return cudaErrorInvalidValue;
-    const size_t smem = PromptSmem<HD, kPpTiles<KVT>>::total + 1024;
+    const size_t smem = PromptSmem<HD, kPpTiles<KVT>, kPpEarly<KVT, HD>>::total + 1024;
     cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<KVT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles<KVT>) + p.r.batch;
