@@ -506,7 +506,10 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         float m = -INFINITY, l = 0.f;
         bool good = true;                        // (a warp whose wait ran out goes on without waiting: its partner's barriers need it)
         if (t < tiles) {
+            // pages all of whose positions all of the warp's rows see: from inner0 on (first positions aside), before inner1
             const int wlow = __reduce_min_sync(0xffffffffu, pos), whigh = __reduce_max_sync(0xffffffffu, pos);
+            const int inner0 = p.window > 0 ? span.sink_pages + max(0, (whigh - p.window + kKvBlock) / kKvBlock - span.first) : 0;
+            const int inner1 = span.sink_pages + (wlow + 1) / kKvBlock - span.first;
             const uint32_t sc = tmem + lanes + t * 128 + half * COLS;
             // Scores: two threads of a row hold theirs in registers, one reads them twice, for the maximum and for the weights.
             constexpr int NG = COLS / 32;
@@ -516,13 +519,8 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 tc_fence_after();
                 tmem_ld32(sc, x[0]);
                 if (HALVES == 2) tmem_ld32(sc + 32, x[1]);
-                // positions that some row of the warp does not see
                 const int v0 = j * kPpPages + half * (kPpPages / 2);
-                bool edge = v0 + kPpPages / HALVES > span.count;
-                if (!edge) {
-                    const int ka = span.page(v0) * kKvBlock, kb = span.page(v0 + kPpPages / HALVES - 1) * kKvBlock + kKvBlock - 1;
-                    edge = kb > wlow || (p.window > 0 && ka <= whigh - p.window && !(kb < p.sinks));
-                }
+                const bool edge = v0 < inner0 || v0 + kPpPages / HALVES > inner1;      // positions that some row of the warp does not see
                 // 32 positions from 32 g on: those that the row does not see to -inf
                 auto hide = [&](uint32_t (&y)[32], int g) {
                     auto below = [](int n) { return (1u << min(max(n, 0), kKvBlock)) - 1u; };
