@@ -291,7 +291,8 @@ int mlb_op_wait_probe(int device, uint32_t max_polls);
  * mlb_ops_status waits for `stream` and reports what the kernels met since the last mlb_ops_status (MLB_E_INVALID: a page
  * id outside the pools, a sequence longer than its row of the page table, a row_start that is no increasing sequence in
  * 0..rows, more rows than max_rows, a position outside the rotation table); what such a sequence should have
- * written is left as it was or, for a bad page id, computed from page 0 (a read) or left out (a write). */
+ * written is left as it was or, for a bad page id, computed from page 0 (a read) or left out (a write). With a row_start that
+ * is no increasing sequence any row of the call may be left as it was. */
 typedef struct mlb_ops mlb_ops;
 int mlb_ops_new(int device, mlb_ops** out);
 void mlb_ops_free(mlb_ops* o);
@@ -302,7 +303,7 @@ int mlb_ops_status(mlb_ops* o, void* stream);
  *   fp4_e2m1: codes [num_pages][kv_heads][16][head_dim / 2] bytes (the even dim in the low half) and e4m3 scales
  *   [num_pages][kv_heads][16][head_dim / 16]; a value is code * scale * k_scale (or v_scale: one positive factor per
  *   pool, so that the scales of its blocks lie well inside e4m3's range; 1 where nothing is known).
- * head_dim 64 or 128. page_table [batch][pt_stride]; entries behind a sequence's last page are not read. */
+ * head_dim 64 or 128, kv_heads up to 65535. page_table [batch][pt_stride]; entries behind a sequence's last page are not read. */
 typedef struct mlb_paged_kv {
     void *kpool, *vpool;
     void *kscale, *vscale;   /* fp4_e2m1 only, else ignored                                 */
@@ -327,7 +328,7 @@ typedef struct mlb_new_rows {
 /* Writes k and v [rows][kv_heads * head_dim] (row_dtype float32 or bfloat16; strides in elements from row to row) to
  * the pages of their positions. With a table rope [rope_len][head_dim] of interleaved (cos, sin) as mlb_rope_table makes
  * it, dims 2i and 2i + 1 of k are turned by the table row of the position first; so is q [rows][heads * head_dim], where
- * given, into q_out (which may be q). Each product and sum of the rotation is one fp32 operation. In a 4-bit cache 16 dims
+ * given, into q_out (which may be q, but not overlap it otherwise). Each product and sum of the rotation is one fp32 operation. In a 4-bit cache 16 dims
  * get the scale e4m3(max|x| / (6 k_scale)) and the codes nearest to x * (1 / (scale * k_scale)), ties to the even code; an
  * infinity takes the largest code and scale, a NaN is stored as some number. Two sequences must not append to one page. */
 int mlb_op_kv_append(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows, int row_dtype, const void* k,
@@ -338,7 +339,7 @@ int mlb_op_kv_read(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows,
                    int64_t k_stride, void* v_out, int64_t v_stride, void* stream);
 /* Causal attention of the rows (already in the cache) over the pages: the row at position p sees position j <= p where
  * window = 0, or j > p - window (its newest `window` positions, itself among them), or j < sinks (the first ones). q and out
- * [rows][heads * head_dim] of row_dtype, heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
+ * [rows][heads * head_dim] of row_dtype (out is not q), heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
  * (0: 1 / sqrt(head_dim)); gate (nullable) fp32 [rows][heads * head_dim] multiplies the output. Sums and softmax statistics are
  * fp32; with float32 rows so is everything else to fp32's own rounding, with bfloat16 rows probabilities may be rounded to bf16. What
  * lies at positions that a row does not see (numbers or not) does not reach its output. */

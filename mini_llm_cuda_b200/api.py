@@ -537,6 +537,8 @@ class Ops:
             qp, qs = self._rows(q, "q", shape, dtype)
             if q_out is q:
                 op, os_ = qp, qs
+            elif q_out is None:
+                raise ValueError("q needs q_out, which may be q itself")
             else:
                 op, os_ = self._rows(q_out, "q_out", shape, dtype)
         rp, rl = None, 0

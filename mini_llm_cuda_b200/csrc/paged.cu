@@ -17,7 +17,7 @@ struct mlb_ops {
 namespace {
 
 constexpr size_t kOpsErrBytes = 256;
-constexpr int kOpsMaxBatch = 4096;
+constexpr int kOpsMaxBatch = 4096, kOpsMaxHeads = 65535;      // (of K/V: a dimension of a grid)
 constexpr size_t kOpsPlanBytes = ((kOpsMaxBatch + 1) * 8 + 255) / 256 * 256;
 
 // The handle's device is current while an object of this lives.
@@ -53,6 +53,7 @@ int check_cache(const char* op, const mlb_paged_kv* kv, const mlb_new_rows* r, i
     }
     if (kv->pt_stride < 1 || kv->num_pages < 1 || kv->kv_heads < 1) return fail(MLB_E_INVALID, "%s: pt_stride, num_pages and kv_heads must be >= 1", op);
     if (kv->pt_stride > (1 << 26)) return fail(MLB_E_UNSUPPORTED, "%s: pt_stride above 2^26 (positions are 31-bit numbers)", op);
+    if (kv->kv_heads > kOpsMaxHeads) return fail(MLB_E_UNSUPPORTED, "%s: kv_heads above %d", op, kOpsMaxHeads);
     if (kv->head_dim != 64 && kv->head_dim != 128) return fail(MLB_E_UNSUPPORTED, "%s: head_dim must be 64 or 128", op);
     if ((reinterpret_cast<uintptr_t>(kv->kpool) | reinterpret_cast<uintptr_t>(kv->vpool)) & 15) return fail(MLB_E_INVALID, "%s: pools start on 16 bytes", op);
     if (kv->dtype == MLB_DT_FP4_E2M1 && ((reinterpret_cast<uintptr_t>(kv->kscale) | reinterpret_cast<uintptr_t>(kv->vscale)) & 15))
@@ -408,6 +409,7 @@ extern "C" int mlb_op_kv_append(mlb_ops* o, const mlb_paged_kv* kv, const mlb_ne
     if (rope_or_null && (rope_len < 1 || reinterpret_cast<uintptr_t>(rope_or_null) % 4)) return fail(MLB_E_INVALID, "append: a rotation table has rows of fp32");
     if (q_or_null) {
         if (heads < 1) return fail(MLB_E_INVALID, "append: heads must be >= 1");
+        if (heads > 8 * kOpsMaxHeads) return fail(MLB_E_UNSUPPORTED, "append: heads above %d", 8 * kOpsMaxHeads);
         if ((rc = check_rows("append", "q", q_or_null, q_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
         if ((rc = check_rows("append", "q_out", q_out, q_out_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
     }
@@ -464,6 +466,7 @@ extern "C" int mlb_op_attn_paged(mlb_ops* o, const mlb_paged_kv* kv, const mlb_n
     if ((rc = check_rows("paged attention", "out", out, out_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
     if (gate_or_null && reinterpret_cast<uintptr_t>(gate_or_null) % 4) return fail(MLB_E_INVALID, "paged attention: gate is not on its type's boundary");
     if ((rc = check_count("paged attention", o, rows, heads, kv->head_dim))) return rc;
+    if (rows->rows > 0 && q == out) return fail(MLB_E_INVALID, "paged attention: out may not be q");
     if (rows->rows == 0) return MLB_OK;
     AttnPagedParams p{};
     p.c = cache_of(kv);

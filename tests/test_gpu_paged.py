@@ -616,3 +616,106 @@ def test_same_answer_as_the_decode_operator(api, ops):
                                       pos.data_ptr(), c.q.data_ptr(), None, ref.data_ptr(), 4, 8, 2, 128, 3, None)
     assert rc == 0
     assert float((out - ref).abs().max()) < 2e-5
+
+
+# ---- sizes at which the work is dealt out in another way ---------------------------------------------------------------
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("batch,kv_heads", [(40, 2), (300, 1), (700, 2)])
+def test_short_sequences_beside_long_ones(api, ops, cache, rows, batch, kv_heads):
+    """Batches on both sides of a CTA's 256 threads, few and many items for each CTA; shares with several short items, long items in many shares."""
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, 60, size=batch)
+    lens[rng.integers(0, batch, size=3)] = rng.integers(2000, 6000, size=3)
+    c = Case(api, [1] * batch, lens.tolist(), 4 * kv_heads, kv_heads, 64, cache, rows, ragged=False)
+    for window, sinks in ((0, 0), (700, 20)):
+        check(attend(ops, c, window, sinks), *c.attention(window, sinks))
+    ops.status()
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd", [(3, 1, 64), (16, 4, 128), (12, 12, 64)])
+def test_append_of_many_rows(api, ops, cache, rows, heads, kv_heads, hd):
+    """Several rows for a CTA: the same bits as sequence by sequence, a row for a CTA each."""
+    import torch
+    new, lens = [900, 0, 1, 1100, 3, 57, 1000, 640, 1013], [900, 7, 1, 1500, 2, 57, 1300, 640, 1020]
+    for steps in (1, 4):
+        n, L = (new, lens) if steps == 1 else ([x * 4 for x in new], [x * 4 for x in lens])
+        c, d = (Case(api, n, L, heads, kv_heads, hd, cache, rows, extra_rows=5) for _ in range(2))
+        rope = rope_table(max(L), hd)
+        q_out, q_ref = torch.full_like(c.q, 777.0), torch.full_like(c.q, 777.0)
+        outs, refs = ([torch.full_like(c.k, 777.0) for _ in range(2)] for _ in range(2))
+        ops.kv_append(c.kv, c.nr, c.k, c.v, rope=rope, q=c.q, q_out=q_out, heads=heads)
+        ops.kv_read(c.kv, c.nr, *outs)
+        t = 0
+        for b, (m, length) in enumerate(zip(n, L)):
+            for i in range(0, m, 500):
+                k = min(500, m - i)
+                kv = api.PagedKV(d.kpool, d.vpool, d.table[b:b + 1].contiguous(), kscale=d.kscale, vscale=d.vscale, k_scale=d.k_scale, v_scale=d.v_scale)
+                nr = api.NewRows(torch.tensor([length - m + i + k], dtype=torch.int32, device="cuda"), k,
+                                 row_start=torch.tensor([0, k], dtype=torch.int32, device="cuda"))
+                s = slice(t + i, t + i + k)
+                ops.kv_append(kv, nr, d.k[s], d.v[s], rope=rope, q=d.q[s], q_out=q_ref[s], heads=heads)
+                ops.kv_read(kv, nr, refs[0][s], refs[1][s])
+            t += m
+        ops.status()
+        assert bool((q_out == q_ref).all())
+        for one in ["kpool", "vpool"] + (["kscale", "vscale"] if cache == "fp4" else []):
+            assert bool((getattr(c, one).view(torch.uint8) == getattr(d, one).view(torch.uint8)).all()), one
+        for x, y in zip(outs, refs):
+            assert bool((x == y).all())
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+def test_calls_in_a_row(api, ops, cache, rows):
+    """Calls of one handle behind one another, none waited for: each has the scratch to itself."""
+    cases = [Case(api, [1, 200, 1, 40], [4000, 300, 77, 2000], 8, 2, 64, cache, rows, seed=1), Case(api, [1] * 70, [500] * 70, 8, 2, 128, cache, rows, ragged=False, seed=2),
+             Case(api, [3, 1], [9000, 6000], 8, 2, 128, cache, rows, seed=3)]
+    alone = [attend(ops, c, 900, 4) for c in cases]
+    ops.status()
+    for c, out in zip(cases, alone):
+        check(out, *c.attention(900, 4))
+    for _ in range(5):
+        again = [attend(ops, c, 900, 4) for c in cases]
+        for a, b in zip(alone, again):
+            assert bool((a == b).all())
+    ops.status()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "fp4", "f32"])
+def test_captured_prompts(api, ops, cache):
+    """Prompts beside single tokens, captured once and replayed with other lengths and row counts within the same rows."""
+    import torch
+    c = Case(api, [1, 300, 4, 90], [700, 900, 350, 95], 8, 2, 64, cache, "bf16", extra_rows=3)
+    c.describe()
+    out = torch.empty_like(c.q)
+    s = torch.cuda.Stream()
+    ops.attn_paged(c.kv, c.nr, c.q, out, heads=8, window=333, sinks=9)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out.fill_(777.0)
+        ops.attn_paged(c.kv, c.nr, c.q, out, heads=8, window=333, sinks=9, stream=torch.cuda.current_stream().cuda_stream)
+    for new, lens in (([1, 300, 4, 90], [700, 900, 350, 95]), ([100, 1, 200, 0], [600, 20, 201, 3]), ([1, 1, 1, 1], [1, 2, 3, 17]), ([0, 0, 0, 398], [5, 5, 5, 96 - 1])):
+        if lens[3] < new[3]:
+            lens[3] = 95                          # rows before position 0 are zeros
+        c.new, c.lens = new, lens
+        c.row_start.copy_(torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32))
+        c.kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        for _ in range(2):
+            g.replay()
+        torch.cuda.synchronize()
+        check(out, *c.attention(333, 9))
+    ops.status()
+    del g
+
+
+def test_out_is_not_q(api, ops):
+    import torch
+    c = Case(api, [1, 2], [5, 6], 4, 2, 64)
+    with pytest.raises(api.MlbError, match="may not be q"):
+        ops.attn_paged(c.kv, c.nr, c.q, c.q, heads=4)
+    with pytest.raises(ValueError, match="q_out"):
+        ops.kv_append(c.kv, c.nr, c.k, c.v, q=c.q, heads=4)
+    with pytest.raises(api.MlbError, match="stride"):
+        ops.kv_append(c.kv, c.nr, c.k[:1].expand(3, -1), c.v)
+    assert torch.cuda.current_device() == 0

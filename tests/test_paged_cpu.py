@@ -118,3 +118,10 @@ def test_no_device(api):
     h = C.c_void_p()
     assert api.lib().mlb_ops_new(0, C.byref(h)) == api.MLB_E_CUDA
     assert not h.value
+
+
+def test_refused_head_counts(api):
+    assert calls(api, cache(api, kv_heads=65536), new_rows(api), stride=1 << 24) == [api.MLB_E_UNSUPPORTED] * 3
+    L, kv, rows, p = api.lib(), cache(api), new_rows(api), 1 << 20
+    assert L.mlb_op_kv_append(None, C.byref(kv), C.byref(rows), api.DT_BF16, p, 4096, p, 4096, None, 0, p, 1 << 30, p, 1 << 30, 8 * 65535 + 1, None) \
+        == api.MLB_E_UNSUPPORTED
