@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_move_kernel(const __grid_c
                 if (in && !pooled) store8(dst + i * p.q_out_stride, vec, x);
             };
             // several rows at a time, so that the loads of all are on their way
-            constexpr int U = 8 / sizeof(RT);
+            constexpr int U = 4;
             for (int i = 0; i < n; i += U) {
                 Raw8<RT> raw[U];
 #pragma unroll
