@@ -15,7 +15,7 @@ namespace {
 // A warp takes pages of 16 positions of one K/V head for a block of up to 8 rows (new tokens x the query heads of the K/V head):
 //   S[16 positions][8 rows] = K Q^T      A = K, B = Q^T,  m16n8k16
 //   O^T[dims][8 rows] += V^T P^T         A = V^T, B = P^T
-// Nothing is staged in shared memory but Q: dims of a dot product and positions of a sum may come in any order, so a lane loads 16
+// fp32 and bf16 pages go straight to registers: dims of a dot product and positions of a sum may come in any order, so a lane loads 16
 // bytes of a K row and uses them as its elements of two (fp32: one, 4 bits: eight) k-steps, and 16 bytes each of four V rows whose
 // 16-bit halves it pairs up with byte permutes. S lies with positions along the lanes and rows within them, as O does: a running maximum
 // and its rescaling need no exchange between lanes but the maximum itself, and that only when a score passes the old one by 2^8; P is
@@ -575,7 +575,10 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
 // ---- the positions of all sequences dealt out evenly ---------------------------------------------------------------------
 // Page counts of a batch's sequences differ, and so does how many sequences there are for 148 SMs: so the pages of all (sequence, K/V
 // head, block of rows) are laid end to end and cut into as many equal shares as there are teams (a CTA's warps together, or each warp alone),
-// and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Sequences of more than
+// and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Bound by HBM with many bf16 pages: 64 sequences in
+// a window of 4096, 32 / 8 heads of 128, 164 us for 932 MB, 87 % of the measured copy rate. By the instructions that widen the codes with 4-bit
+// pages: 128 sequences of up to 8000 positions, the same heads, 139 us for 602 MB, 66 %. By latency (lengths, queries, page ids, pages, the
+// CTA's results, the join: some 2 us each) with few: one user in a window of 1024, 11 us. Sequences of more than
 // kSplitRows (token, head) pairs are left to the kernels for prompts.
 // (sequences, pages of their items before them) -> plan in shared memory; returns the total
 __device__ __forceinline__ int split_blocks(const AttnPagedParams& p, int n) {
@@ -985,9 +988,11 @@ cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int ctas = 2 * sm_count;
     p.max_teams = TEAM == 1 ? ctas * kSplitWarps : ctas;
-    // Beside its pages an item costs what comes before and after them, about as much as two pages of each of its team's warps. Where a share has parts of two
-    // items at most, each of its CTA's own, that is the same for all and left out.
-    p.item_cost = (long long)p.r.batch * p.c.kv_heads * 4 >= p.max_teams ? 2 * TEAM : 0;
+    // Beside its pages an item costs what comes before and after them, measured in pages: 7 small ones of 4 bits for a warp alone (2: 153 us for 128
+    // sequences of up to 8000 positions, 4: 146, 6: 140, 8: 138; 256 short ones 63, 52, 47, 46), 4 others (2: 86 us for 200 sequences of up to 2000, 4:
+    // 81, 8: 84), and two for each warp of a team (1: 172 us for 64 sequences in a window of 4096, 2: 164, 4: 166). Where a share has parts of two items at
+    // most, that is the same for all and left out.
+    p.item_cost = (long long)p.r.batch * p.c.kv_heads * 4 < p.max_teams ? 0 : TEAM > 1 ? 2 * TEAM : sizeof(KVT) == 1 ? 7 : 4;
     attn_split_kernel<KVT, RT, HD, TEAM><<<ctas, 32 * kSplitWarps, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const int blocks = p.r.row_start ? kSplitRows / 8 : 1;
