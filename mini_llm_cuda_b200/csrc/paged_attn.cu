@@ -599,12 +599,46 @@ struct Shares {
         each = div(total, teams);
         more = (unsigned)(total - each * teams);
     }
+    // of `size` each, of a total that is so many of them
+    __device__ __forceinline__ Shares(unsigned long long total, unsigned size) : each(size), teams((unsigned)div(total, size)), more(0) {}
     __device__ __forceinline__ unsigned long long start(unsigned t) const { return each * t + min(t, more); }
     __device__ __forceinline__ unsigned holder(unsigned long long x) const {         // of x < total
         const unsigned long long big = (each + 1) * more;
         return x < big ? (unsigned)div(x, each + 1) : more + (unsigned)div(x - big, each);
     }
 };
+
+// Units of an item in the plan: pages and what p.item_cost adds; with few items (`size` > 0) pages up to a multiple of the shares' size, so that no
+// share has parts of two items (that one ended 5 us after the others).
+__device__ __forceinline__ unsigned item_units(const AttnPagedParams& p, unsigned size, int pages) {
+    const unsigned n = (unsigned)max(1, pages + p.item_cost);
+    return size > 0 ? (n + size - 1) / size * size : n;
+}
+// The size of a share, 0 where items are many: with at most one share more for every item there are no more than p.max_teams. Called by all of a
+// CTA's threads; a sequence for each of them, since there are fewer than p.max_teams / 4 items.
+template <int TEAM>
+__device__ __forceinline__ unsigned share_size(const AttnPagedParams& p, unsigned long long (&sums)[2][kSplitWarps]) {
+    if (p.item_cost > 0) return 0;
+    unsigned long long n = 0, items = 0;
+    if ((int)threadIdx.x < p.r.batch) {
+        const PagedSeq s = paged_seq(p.r, p.c.pt_stride, threadIdx.x, false);
+        items = (unsigned long long)split_blocks(p, s.n) * p.c.kv_heads;
+        if (items > 0) n = item_units(p, 0, paged_span(p, s.len - s.n, s.len - 1).count) * items;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+        items += __shfl_xor_sync(0xffffffffu, items, o);
+    }
+    if (threadIdx.x % 32 == 0) { sums[0][threadIdx.x / 32] = n; sums[1][threadIdx.x / 32] = items; }
+    __syncthreads();
+    n = items = 0;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) { n += sums[0][w]; items += sums[1][w]; }
+    __syncthreads();
+    const unsigned teams = (unsigned)p.max_teams - (unsigned)items;
+    return max((unsigned)TEAM, (unsigned)Shares::div(n + teams - 1, teams));
+}
 
 // TEAM: warps of a team, 1 or kSplitWarps
 template <typename KVT, typename RT, int HD, int TEAM>
@@ -616,10 +650,11 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
     float* red = reinterpret_cast<float*>(ring);                                         // TEAM > 1: [warp][8][W], a row's maximum and total behind its sums
     unsigned long long* plan = reinterpret_cast<unsigned long long*>(ring + split_ring_bytes<KVT, HD, TEAM>());      // [batch + 1]
     __shared__ float qs_all[kSplitWarps][8];
-    __shared__ unsigned long long warp_sum_[kSplitWarps];
+    __shared__ unsigned long long warp_sum_[kSplitWarps], sums[2][kSplitWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
     pdl_launch_dependents();
-    // pages before each sequence
+    const unsigned size = share_size<TEAM>(p, sums);
+    // units before each sequence
     unsigned long long before = 0;
     for (int b0 = 0; b0 < p.r.batch; b0 += 32 * kSplitWarps) {
         const int b = b0 + tid;
@@ -627,7 +662,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         if (b < p.r.batch) {
             const PagedSeq s = paged_seq(p.r, p.c.pt_stride, b, blockIdx.x == 0);
             const int blocks = split_blocks(p, s.n);
-            if (blocks > 0) n = (unsigned long long)max(1, p.item_cost + paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
+            if (blocks > 0) n = (unsigned long long)item_units(p, size, paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
         }
         unsigned long long x = n;
 #pragma unroll
@@ -653,7 +688,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         for (int b = tid; b <= p.r.batch; b += 32 * kSplitWarps) p.plan[b] = plan[b];
     const unsigned long long total = before;
     if (total == 0) return;
-    const Shares shares(total, p.max_teams, TEAM + p.item_cost);
+    const Shares shares = size > 0 ? Shares(total, size) : Shares(total, p.max_teams, TEAM + p.item_cost);
     const unsigned team = TEAM == 1 ? blockIdx.x * kSplitWarps + warp : blockIdx.x;
     if (team >= shares.teams) return;
     const unsigned long long start = shares.start(team), end = shares.start(team + 1);
@@ -672,7 +707,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         k.s = paged_seq(p.r, p.c.pt_stride, b, false);
         const int blocks = split_blocks(p, k.s.n);
         const PagedSpan span = paged_span(p, k.s.len - k.s.n, k.s.len - 1);
-        const unsigned count = (unsigned)max(1, span.count + p.item_cost);
+        const unsigned count = item_units(p, size, span.count);
         const unsigned long long rest = at - plan[b], left = end - at, item64 = Shares::div(rest, count);
         const unsigned c0 = (unsigned)(rest - item64 * count), c1 = left < count - c0 ? c0 + (unsigned)left : count, item = (unsigned)item64;
         const int v0 = max(0, (int)c0 - p.item_cost), v1 = max(0, (int)c1 - p.item_cost);      // pages
@@ -774,6 +809,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __gri
     const int i = WPR == 1 ? warp : (int)blockIdx.y;
     pdl_launch_dependents();
     // Where the item lies in the plan, while the other kernel is at work: worked out again where a thread has one sequence at most, else read
+    const unsigned size = share_size<TEAM>(p, sums);
     unsigned long long total = 0, o0 = 0;
     const bool own_plan = p.r.batch <= 32 * kSplitWarps;
     if (own_plan) {
@@ -781,7 +817,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __gri
         if ((int)threadIdx.x < p.r.batch) {
             const PagedSeq s = paged_seq(p.r, p.c.pt_stride, threadIdx.x, false);
             const int blocks = split_blocks(p, s.n);
-            if (blocks > 0) n = (unsigned long long)max(1, p.item_cost + paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
+            if (blocks > 0) n = (unsigned long long)item_units(p, size, paged_span(p, s.len - s.n, s.len - 1).count) * blocks * p.c.kv_heads;
         }
         unsigned long long before = (int)threadIdx.x < b ? n : 0;
 #pragma unroll
@@ -811,9 +847,9 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __gri
         if (own_plan) pdl_wait();
         return;
     }
-    const unsigned count = (unsigned)max(1, paged_span(p, k.s.len - k.s.n, k.s.len - 1).count + p.item_cost);
+    const unsigned count = item_units(p, size, paged_span(p, k.s.len - k.s.n, k.s.len - 1).count);
     o0 += (unsigned long long)item * count;
-    const Shares shares(total, p.max_teams, TEAM + p.item_cost);
+    const Shares shares = size > 0 ? Shares(total, size) : Shares(total, p.max_teams, TEAM + p.item_cost);
     const unsigned t0 = shares.holder(o0), t1 = shares.holder(o0 + count - 1), slot0 = shares.start(t0) == o0 ? 0 : 1;
     if (own_plan) pdl_wait();
     if (t0 == t1) return;                        // one team held it all and wrote the result
