@@ -578,7 +578,7 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
 // and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Bound by HBM with many bf16 pages: 64 sequences in
 // a window of 4096, 32 / 8 heads of 128, 164 us for 932 MB, 87 % of the measured copy rate. By the instructions that widen the codes with 4-bit
 // pages: 128 sequences of up to 8000 positions, the same heads, 139 us for 602 MB, 66 %. By latency (lengths, queries, page ids, pages, the
-// CTA's results, the join: some 2 us each) with few: one user in a window of 1024, 11 us. Sequences of more than
+// CTA's results, the join: some 1 to 2 us each) with few: one user in a window of 1024, 9 us. Sequences of more than
 // kSplitRows (token, head) pairs are left to the kernels for prompts.
 // (sequences, pages of their items before them) -> plan in shared memory; returns the total
 __device__ __forceinline__ int split_blocks(const AttnPagedParams& p, int n) {
