@@ -11,7 +11,7 @@
 // Positions that no row of the CTA sees (behind the last one, between the first positions and the window) are zeros in V: 0 times what
 // may lie there could be no number. A row whose result is not finite is done again from the formula (careful_row).
 //
-// What bounds it (bf16, heads of 128): not the tensor core (43 % of its cycles), the exponential's unit (33 %) or the issue slots (37 %), but the chain
+// What bounds it (bf16, heads of 128): not the tensor core (36 % of its cycles in the window below), the exponential's unit (32 %) or the issue slots (46 %), but the chain
 // softmax -> P V -> next scores of each tile, 3500 cycles of which two tiles overlap; tensor memory holds no third tile and no second S. 8001
 // tokens, 16 / 4 heads of 128: 262 us, 1000 TFLOP/s; in a window of 1024 104 us, 590 TFLOP/s, where a CTA's start and end (6 us of 26) tell.
 #include <cstring>
