@@ -341,7 +341,8 @@ int mlb_op_kv_read(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows,
  * window = 0, or j > p - window (its newest `window` positions, itself among them), or j < sinks (the first ones). q and out
  * [rows][heads * head_dim] of row_dtype (out is not q), heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
  * (0: 1 / sqrt(head_dim)); gate (nullable) fp32 [rows][heads * head_dim] multiplies the output. Sums and softmax statistics are
- * fp32; with float32 rows so is everything else to fp32's own rounding, with bfloat16 rows probabilities may be rounded to bf16. What
+ * fp32; with float32 rows so is everything else to fp32's own rounding (over 4-bit pages q is taken to 22 bits, and to no finer than 2^-33 of
+ * its row's largest), with bfloat16 rows probabilities may be rounded to bf16: each of them, however small beside the largest. What
  * lies at positions that a row does not see (numbers or not) does not reach its output. */
 int mlb_op_attn_paged(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows, int row_dtype, const void* q,
                       int64_t q_stride, const float* gate_or_null, void* out, int64_t out_stride, int heads, float scale,

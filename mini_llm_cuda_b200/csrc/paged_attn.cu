@@ -20,9 +20,13 @@ namespace {
 // 16-bit halves it pairs up with byte permutes. S lies with positions along the lanes and rows within them, as O does: a running maximum
 // and its rescaling need no exchange between lanes but the maximum itself, and that only when a score passes the old one by 2^8; P is
 // turned round by movmatrix.
-// fp32 numbers are taken in pieces whose products are exact: an fp32 query in three bf16 (4-bit pages: two halves, the row scaled by
-// a power of two to lie within their range), fp32 K and V in three bf16, a probability in as many as the rows' type needs. Products of
-// pieces below 2^-24 of the whole are left out. 4-bit codes times their e4m3 scale are exact halves.
+// fp32 numbers are taken in pieces whose products are exact: fp32 queries, K, V and probabilities in three bf16, probabilities of bf16 rows in two (4-bit pages: one). Products of
+// pieces below 2^-24 of the whole are left out. 4-bit codes times their e4m3 scale are exact halves, to which the conversion instruction brings them, and meet
+// queries as halves (fp32: two of them, bf16: one), the row scaled by a power of two to lie within their range.
+// Probabilities are in bf16 and not in halves over 4-bit pages too, where the codes of V are widened to bf16 for them: a probability may have any magnitude, and
+// where one position outweighs the rest and brings next to nothing (the first one does both in trained models) the answer is what the rest add up to; halves
+// have 11 bits from 2^-14 on only. 128 sequences of up to 8000 positions, bf16 rows: 158 us, in halves 139, in two pieces 174. (Halves in bands of 2^24, those
+// below the first weighed by themselves: 150, and up to 190 where scores lie far apart.)
 constexpr int kSplitWarps = 8;
 constexpr float kLazy = 8.f;         // log2 of how far a score may pass the running maximum before it is moved
 
@@ -54,15 +58,15 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
     return y;
 }
-// N bf16 (or half) pairs whose sum is the pair (x, y) to 8 N (11 N) bits
-template <bool F16, int N>
+// N bf16 (or half) pairs whose sum is the pair (x, y) to 8 N bits (11 N, of halves no finer than 2^-25)
+template <bool HALF = false, int N>
 __device__ __forceinline__ void pieces(float x, float y, uint32_t (&o)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        o[i] = F16 ? f32x2_to_f16(x, y) : f32x2_to_bf16(x, y);
+        o[i] = HALF ? f32x2_to_f16(x, y) : f32x2_to_bf16(x, y);
         if (i + 1 < N) {
-            x -= F16 ? f16_lo(o[i]) : __uint_as_float(o[i] << 16);
-            y -= F16 ? f16_hi(o[i]) : __uint_as_float(o[i] & 0xffff0000u);
+            x -= HALF ? f16_lo(o[i]) : __uint_as_float(o[i] << 16);
+            y -= HALF ? f16_hi(o[i]) : __uint_as_float(o[i] & 0xffff0000u);
         }
     }
 }
@@ -74,7 +78,7 @@ template <typename KVT, int HD> struct PageFrag;
 template <int HD>
 struct PageFrag<bf16_t, HD> {
     static constexpr int KP = 1;                             // pieces of K and V
-    static constexpr bool F16 = false;
+    static constexpr bool Q4 = false;
     uint4 k[2][HD / 32], v[HD / 64][4];
     __device__ static int dim(int ks, int j, int slot) { return ks / 2 * 32 + j * 8 + ks % 2 * 4 + slot; }
     __device__ static int vdim(int mt, int g) { return mt / 4 * 64 + g * 8 + mt % 4 * 2; }
@@ -113,7 +117,7 @@ struct PageFrag<bf16_t, HD> {
 template <int HD>
 struct PageFrag<float, HD> {
     static constexpr int KP = 3;
-    static constexpr bool F16 = false;
+    static constexpr bool Q4 = false;
     float4 k[2][HD / 16], v[HD / 32][4];
     __device__ static int dim(int ks, int j, int slot) { return ks * 16 + j * 4 + slot; }
     __device__ static int vdim(int mt, int g) { return mt / 2 * 32 + g * 4 + mt % 2 * 2; }
@@ -137,10 +141,10 @@ struct PageFrag<float, HD> {
     }
     __device__ __forceinline__ void k_operand(int ks, uint32_t (&a)[3][4]) const {
         uint32_t w[4][3];
-        pieces<false, 3>(k[0][ks].x, k[0][ks].y, w[0]);
-        pieces<false, 3>(k[1][ks].x, k[1][ks].y, w[1]);
-        pieces<false, 3>(k[0][ks].z, k[0][ks].w, w[2]);
-        pieces<false, 3>(k[1][ks].z, k[1][ks].w, w[3]);
+        pieces(k[0][ks].x, k[0][ks].y, w[0]);
+        pieces(k[1][ks].x, k[1][ks].y, w[1]);
+        pieces(k[0][ks].z, k[0][ks].w, w[2]);
+        pieces(k[1][ks].z, k[1][ks].w, w[3]);
 #pragma unroll
         for (int i = 0; i < 3; ++i)
 #pragma unroll
@@ -152,7 +156,7 @@ struct PageFrag<float, HD> {
         for (int h = 0; h < 4; ++h) {                        // a0, a1: keys 2j, 2j + 1 of the two dims; a2, a3: keys 2j + 8, 2j + 9
             const float4 &x = v[mt / 2][h / 2 * 2], &y = v[mt / 2][h / 2 * 2 + 1];
             const float u = mt % 2 ? (h % 2 ? x.w : x.z) : (h % 2 ? x.y : x.x), z = mt % 2 ? (h % 2 ? y.w : y.z) : (h % 2 ? y.y : y.x);
-            pieces<false, 3>(u, z, w[h]);
+            pieces(u, z, w[h]);
         }
 #pragma unroll
         for (int i = 0; i < 3; ++i)
@@ -163,7 +167,8 @@ struct PageFrag<float, HD> {
 
 template <int HD>
 struct PageFrag<fp4_t, HD> {
-    static constexpr bool F16 = true;
+    static constexpr int KP = 1;
+    static constexpr bool Q4 = true;
     static constexpr int KW = HD / 32, VW = HD / 64;         // words of codes of a K row per lane, of a V row
     uint32_t k[2][KW], ks_[2], v[4][VW], vs[2];
     __device__ static int dim(int ks, int j, int slot) { return j * (HD / 4) + ks * 4 + slot; }
@@ -242,7 +247,7 @@ __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const ui
     using F = PageFrag<KVT, HD>;
     float t[4] = {0.f, 0.f, 0.f, 0.f};                       // two chains of products
     s[0] = s[1] = s[2] = s[3] = 0.f;
-    if constexpr (F::F16) {
+    if constexpr (F::Q4) {
         uint32_t h[2][HD / 8];
         f.widen_k(h);
 #pragma unroll
@@ -270,35 +275,30 @@ __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const ui
     for (int e = 0; e < 4; ++e) s[e] += t[e];
 }
 
-// acc[mt]: dims vdim(mt, g) of rows 2j, 2j + 1 in [0], [1], the next dim in [2], [3]
+// acc[mt]: dims vdim(mt, g) of rows 2j, 2j + 1 in [0], [1], the next dim in [2], [3] (4-bit pages: a 256th of them, as widen_codes has it)
 template <typename KVT, int HD, int PP>
 __device__ __forceinline__ void page_values(const PageFrag<KVT, HD>& f, const float (&w)[4], float (&acc)[HD / 16][4]) {
     using F = PageFrag<KVT, HD>;
     uint32_t p0[PP], p1[PP];
-    pieces<F::F16, PP>(w[0], w[1], p0);
-    pieces<F::F16, PP>(w[2], w[3], p1);
+    pieces(w[0], w[1], p0);
+    pieces(w[2], w[3], p1);
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
         p0[i] = movmatrix(p0[i]);
         p1[i] = movmatrix(p1[i]);
     }
-    if constexpr (F::F16) {
-        const uint32_t s0 = e4m3x2_to_f16(f.vs[0]), s1 = e4m3x2_to_f16(f.vs[1]);
+    if constexpr (F::Q4) {
+        const uint32_t h0 = e4m3x2_to_f16(f.vs[0]), h1 = e4m3x2_to_f16(f.vs[1]);
+        const uint32_t s0 = f32x2_to_bf16(f16_lo(h0) * kScaleUp, f16_hi(h0) * kScaleUp), s1 = f32x2_to_bf16(f16_lo(h1) * kScaleUp, f16_hi(h1) * kScaleUp);
 #pragma unroll
-        for (int w8 = 0; w8 < F::VW; ++w8) {
-            // codes of one dim and two neighbouring rows side by side, of even dims, of odd ones
-            uint32_t h[4][4];
+        for (int w = 0; w < 2 * F::VW; ++w) {
+            // four dims of two neighbouring rows, the one's codes under the other's: widen_codes puts a dim's two together
+            const int sel = w % 2 ? 0x7632 : 0x5410;
+            const uint4 x = widen_codes(__byte_perm(f.v[0][w / 2], f.v[1][w / 2], sel), s0), y = widen_codes(__byte_perm(f.v[2][w / 2], f.v[3][w / 2], sel), s1);
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const uint32_t x = f.v[i][w8], y = f.v[i + 1][w8];
-                e2m1x8_to_f16((x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u), h[i]);
-                e2m1x8_to_f16((x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), h[i + 1]);
-            }
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const uint32_t a0 = hmul2(h[0][m], s0), a1 = hmul2(h[1][m], s0), a2 = hmul2(h[2][m], s1), a3 = hmul2(h[3][m], s1);
-#pragma unroll
-                for (int i = 0; i < PP; ++i) mma_f16(acc[w8 * 4 + m], a0, a1, a2, a3, p0[i], p1[i]);
+            for (int i = 0; i < PP; ++i) {
+                mma_bf16(acc[w * 2], x.x, x.y, y.x, y.y, p0[i], p1[i]);
+                mma_bf16(acc[w * 2 + 1], x.z, x.w, y.z, y.w, p0[i], p1[i]);
             }
         }
     } else {
@@ -321,7 +321,7 @@ struct Block {
     PagedSeq s;
 };
 
-template <typename RT, bool F16, int QP, int HD, typename F>
+template <typename RT, int QP, int HD, typename F>
 __device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Block& k, uint2* qf, float* qscale, int lane) {
     const int g = lane >> 2, j = lane & 3;                   // the B operand's column is a row of the block
     const bool in = g < k.count;
@@ -349,7 +349,7 @@ __device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Blo
         }
     }
     float up = 1.f, down = 1.f;
-    if (F16) {
+    if (F::Q4) {
         // a power of two that brings the row's largest magnitude to 256 .. 512, if it is a number
         float top = 0.f;
 #pragma unroll
@@ -366,8 +366,8 @@ __device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Blo
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
         uint32_t lo[QP], hi[QP];
-        pieces<F16, QP>(x[ks][0] * up, x[ks][1] * up, lo);
-        pieces<F16, QP>(x[ks][2] * up, x[ks][3] * up, hi);
+        pieces<F::Q4>(x[ks][0] * up, x[ks][1] * up, lo);
+        pieces<F::Q4>(x[ks][2] * up, x[ks][3] * up, hi);
 #pragma unroll
         for (int i = 0; i < QP; ++i) qf[(i * (HD / 16) + ks) * 32 + lane] = make_uint2(lo[i], hi[i]);
     }
@@ -376,8 +376,8 @@ __device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Blo
 template <typename KVT, typename RT, int HD>
 struct SplitShape {
     using F = PageFrag<KVT, HD>;
-    static constexpr int QP = sizeof(RT) == 2 ? 1 : F::F16 ? 2 : 3;
-    static constexpr int PP = sizeof(RT) == 2 ? (F::F16 ? 1 : 2) : F::F16 ? 2 : 3;
+    static constexpr int QP = sizeof(RT) == 2 ? 1 : F::Q4 ? 2 : 3;
+    static constexpr int PP = sizeof(RT) == 4 ? 3 : F::Q4 ? 1 : 2;
     static constexpr int QWORDS = QP * (HD / 16) * 32;       // uint2 of a warp's queries
     static constexpr int W = HD + 2;                         // floats of a row's partial result: its sums, maximum, total
     static constexpr int PART = 8 * W;
@@ -553,9 +553,9 @@ __device__ __forceinline__ void block_row(const AttnPagedParams& p, const Block&
 }
 
 // Result of dims d, d + 1 of a row: sums over the total. True if it is not finite (a row that sees nothing is 0).
-template <typename RT, int HD>
+template <typename KVT, typename RT, int HD>
 __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int h, int pos, int d, float x, float y, float l) {
-    const float inv = pos < 0 ? 0.f : p.c.v_scale / l;
+    const float inv = pos < 0 ? 0.f : p.c.v_scale * (sizeof(KVT) == 1 ? kCodeScale : 1.f) / l;
     x = pos < 0 ? 0.f : x * inv;
     y = pos < 0 ? 0.f : y * inv;
     const size_t at = (size_t)row * p.heads * HD + (size_t)h * HD + d;
@@ -577,7 +577,7 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
 // head, block of rows) are laid end to end and cut into as many equal shares as there are teams (a CTA's warps together, or each warp alone),
 // and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Bound by HBM with many bf16 pages: 64 sequences in
 // a window of 4096, 32 / 8 heads of 128, 164 us for 932 MB, 87 % of the measured copy rate. By the instructions that widen the codes with 4-bit
-// pages: 128 sequences of up to 8000 positions, the same heads, 139 us for 602 MB, 66 %. By latency (lengths, queries, page ids, pages, the
+// pages: 128 sequences of up to 8000 positions, the same heads, 159 us for 602 MB, 58 %. By latency (lengths, queries, page ids, pages, the
 // CTA's results, the join: some 1 to 2 us each) with few: one user in a window of 1024, 9 us. Sequences of more than
 // kSplitRows (token, head) pairs are left to the kernels for prompts.
 // (sequences, pages of their items before them) -> plan in shared memory; returns the total
@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         const int mine0 = v0 + (TEAM > 1 ? warp : 0);
         PageSource<KVT, HD> page(p, k, span, mine0, min(v1, span.count), TEAM, ring + warp * PageSource<KVT, HD>::kRing);
         __syncwarp();
-        pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
+        pack_queries<RT, S::QP, HD, typename S::F>(p, k, const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
         __syncwarp();
         float acc[HD / 16][4], m[2], l[2];
         walk_pages<KVT, RT, HD>(p, k, span, mine0, min(v1, span.count), TEAM, page, qf, qscale, acc, m, l);
@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
                     int row, h, pos;
                     block_row(p, k, i, row, h, pos);
 #pragma unroll
-                    for (int t = 0; t < HD / 16; ++t) odd |= put_pair<RT, HD>(p, row, h, pos, S::F::vdim(t, g), acc[t][c], acc[t][2 + c], l[c]);
+                    for (int t = 0; t < HD / 16; ++t) odd |= put_pair<KVT, RT, HD>(p, row, h, pos, S::F::vdim(t, g), acc[t][c], acc[t][2 + c], l[c]);
                 } else {
 #pragma unroll
                     for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<float2*>(part + i * S::W + S::F::vdim(t, g)) = make_float2(acc[t][c], acc[t][2 + c]);
@@ -785,7 +785,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
                 block_row(p, k, i, row, h, pos);
 #pragma unroll
                 for (int e = 0; e < HD / 64; ++e) {
-                    if (whole) odd |= put_pair<RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
+                    if (whole) odd |= put_pair<KVT, RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
                     else *reinterpret_cast<float2*>(part + i * S::W + e * 64 + lane * 2) = o[e];
                 }
                 if (!whole && lane == 0) { part[i * S::W + HD] = mx; part[i * S::W + HD + 1] = lt; }
@@ -918,7 +918,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_join_kernel(const __gri
     block_row(p, k, i, row, h, pos);
     bool odd = false;
 #pragma unroll
-    for (int e = 0; e < HD / 64; ++e) odd |= put_pair<RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
+    for (int e = 0; e < HD / 64; ++e) odd |= put_pair<KVT, RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
     if (__any_sync(0xffffffffu, odd)) careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
 }
 
@@ -973,7 +973,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     const int pos0 = k.s.len - k.s.n;
     const PagedSpan span = paged_span(p, pos0 + k.first / p.group, pos0 + (k.first + k.count - 1) / p.group);
     PageSource<KVT, HD> page(p, k, span, warp, span.count, kSplitWarps, ring + warp * PageSource<KVT, HD>::kRing);
-    if (warp == 0) pack_queries<RT, S::F::F16, S::QP, HD, typename S::F>(p, k, qf, qscale, lane);
+    if (warp == 0) pack_queries<RT, S::QP, HD, typename S::F>(p, k, qf, qscale, lane);
     __syncthreads();
     float acc[HD / 16][4], m[2], l[2];
     walk_pages<KVT, RT, HD>(p, k, span, warp, span.count, kSplitWarps, page, qf, qscale, acc, m, l);
@@ -1012,7 +1012,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     block_row(p, k, i, row, h, pos);
     bool odd = false;
 #pragma unroll
-    for (int e = 0; e < HD / 64; ++e) odd |= put_pair<RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
+    for (int e = 0; e < HD / 64; ++e) odd |= put_pair<KVT, RT, HD>(p, row, h, pos, e * 64 + lane * 2, o[e].x, o[e].y, lt);
     if (__any_sync(0xffffffffu, odd)) careful_row<KVT, RT, HD>(p, k.b, pos, row, h);
 }
 

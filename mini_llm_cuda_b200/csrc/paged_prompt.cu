@@ -159,22 +159,6 @@ struct PromptSmem {
 };
 enum PromptBar { PB_KFULL = 0, PB_KEMPTY = 2, PB_VFULL = 4, PB_VEMPTY = 6, PB_Q = 8, PB_S = 9, PB_P = 11, PB_P2 = 13, PB_O = 15, PB_END = 17, PB_READ = 18, PB_COUNT = 19 };
 
-// 4-bit pages: eight codes (dims 0 .. 7) -> four bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code * scale / 256. Exponent and mantissa of
-// a code are put at the low end of a bf16's exponent, which makes it code * 2^-126 exactly (0.5 as a subnormal), and multiplied by `s`, the
-// block's scale * 2^118 twice. In that order a pair takes two shifts, two logic instructions and a product. (The conversion instruction
-// runs at a quarter of the rate of these and gives halves.)
-__device__ __forceinline__ uint4 widen_codes(uint32_t w, uint32_t s) {
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t sign = i < 3 ? w << (12 - 4 * i) : w, rest = i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6);
-        const uint32_t raw = (sign & 0x80008000u) | (rest & 0x01c001c0u);
-        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(raw), "r"(s));
-    }
-    return make_uint4(r[0], r[1], r[2], r[3]);
-}
-constexpr float kPpCodeScale = 256.f;            // what those values lack
-
 template <typename KVT, int HD>
 __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
     attn_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnPagedParams p) {
@@ -289,7 +273,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
 #pragma unroll
             for (int e = 0; e < CW; e += 4) {                // two scales at a time
                 const uint32_t two = e4m3x2_to_f16(sc[e / 8] >> (e % 8 * 4));
-                const float a = f16_lo(two) * 3.3230699894622897e35f, d = f16_hi(two) * 3.3230699894622897e35f;      // 2^118
+                const float a = f16_lo(two) * kScaleUp, d = f16_hi(two) * kScaleUp;
                 const uint32_t s0 = f32x2_to_bf16(a, a), s1 = f32x2_to_bf16(d, d);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -473,7 +457,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         };
         auto staged = [&](int rl, int ch) { return reinterpret_cast<uint4*>(sm + L::q + t * L::kQ + ch / 8 * L::kHalf + rl * 128 + ((ch % 8) ^ (rl & 7)) * 16); };
         // queries, K-major with the swizzle that the MMA expects; a negative scale turns their sign
-        const float scale = p.scale * p.c.k_scale * (Q4 ? kPpCodeScale : 1.f) * 1.4426950408889634f;
+        const float scale = p.scale * p.c.k_scale * (Q4 ? kCodeScale : 1.f) * 1.4426950408889634f;
         {
             const bf16_t* q = static_cast<const bf16_t*>(p.q);
             const bool vec = ((reinterpret_cast<uintptr_t>(q) | (uint64_t)p.q_stride * 2) & 15) == 0;
@@ -644,7 +628,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                 pair_sync();
                 l = shared_row[t][0][r] + shared_row[t][1][r];   // the same sum in both threads
             }
-            const float inv = pos < 0 ? 0.f : p.c.v_scale * (Q4 ? kPpCodeScale : 1.f) / l;
+            const float inv = pos < 0 ? 0.f : p.c.v_scale * (Q4 ? kCodeScale : 1.f) / l;
             bool odd = false;
             if (good) {
 #pragma unroll 1

@@ -11,6 +11,23 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// 4-bit pages: eight codes (dims 0 .. 7) -> four bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code * scale / 256. Exponent and mantissa of
+// a code are put at the low end of a bf16's exponent, which makes it code * 2^-126 exactly (0.5 as a subnormal), and multiplied by `s`, the
+// block's scale * 2^118 (once for each of a pair). In that order a pair takes two shifts, two logic instructions and a product. (The conversion instruction
+// runs at a quarter of the rate of these and gives halves.)
+__device__ __forceinline__ uint4 widen_codes(uint32_t w, uint32_t s) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t sign = i < 3 ? w << (12 - 4 * i) : w, rest = i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6);
+        const uint32_t raw = (sign & 0x80008000u) | (rest & 0x01c001c0u);
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(raw), "r"(s));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+constexpr float kScaleUp = 3.3230699894622897e35f;      // 2^118
+constexpr float kCodeScale = 256.f;            // what those values lack
+
 // ---- one row, one head, by one warp, straight from the formula --------------------------------------------------------
 // A product with a probability that is not of the row's own positions does not happen here, so infinities and NaN outside of them cannot
 // reach the row, and an infinite score or value gives what the formula gives. The matrix-core kernels redo a row here whose result is

@@ -1,0 +1,85 @@
+"""GPU: paged attention where a few numbers decide the answer: weights over a wide range, every position by itself, positions that hold no numbers."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_paged import TYPES, U, U16, Case, attend
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def api(built_lib):
+    from mini_llm_cuda_b200 import api as _api
+    return _api
+
+
+@pytest.fixture(scope="module")
+def ops(api):
+    return api.Ops(0)
+
+
+# ---- weights over a wide range -----------------------------------------------------------------------------------------
+def first_key_takes_all(c, above):
+    """Scores of about `above` powers of two at position 0 of every sequence, whose value is 0.001, and of -1, 0 or 1 elsewhere: the output is made of
+    the small weights. A score has two products, the rest are zeros."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+    first = c.table[:, 0].long()
+    sign = torch.randint(0, 3, c.kpool.shape[:3], generator=g, device="cuda")
+    c.kpool.zero_()
+    if c.cache == "fp4":
+        c.kscale.copy_(torch.ones(c.kscale.shape, device="cuda"))
+        c.kpool[..., 0] = torch.tensor([0x00, 0x20, 0xa0], dtype=torch.uint8, device="cuda")[sign]      # dim 1: 0, 1, -1
+        c.kpool[first, :, 0, 0] = 0x02                                                                  # dim 0: 1
+        c.vpool[first, :, 0] = 0x11
+        c.vscale[first, :, 0] = torch.full((), 2.0 ** -9, device="cuda").to(torch.float8_e4m3fn)
+    else:
+        c.kpool[..., 1] = (sign - 1).to(c.kpool.dtype)
+        c.kpool[first, :, 0, 1] = 0
+        c.kpool[first, :, 0, 0] = 1
+        c.vpool[first, :, 0] = 0.001
+    q = torch.zeros(c.rows, c.heads, c.hd, device="cuda")
+    q[..., 0] = above * math.log(2) * math.sqrt(c.hd) * (1 + 0.01 * torch.arange(c.heads, device="cuda"))
+    q[..., 1] = 0.7 * math.sqrt(c.hd)
+    c.q = q.flatten(1).to(c.dt)
+
+
+def small_weights(c, out):
+    """Largest error of the output over its bound, relative to the sum of w |v| and not to the largest value."""
+    import torch
+    H, D, KH, worst, r0 = c.heads, c.hd, c.kv_heads, 0.0, 0
+    for b, (n, L) in enumerate(zip(c.new, c.lens)):
+        q = c.q[r0:r0 + n].double().reshape(n, KH, H // KH, D).permute(1, 2, 0, 3)
+        K, V = c.cached("k", b, L), c.cached("v", b, L)
+        hidden = torch.arange(L, device="cuda")[None] > torch.arange(L - n, L, device="cuda")[:, None]
+        s = (q @ K[:, None].transpose(-1, -2) / math.sqrt(D)).masked_fill(hidden, -math.inf)
+        w = torch.softmax(s, dim=-1)
+        o, size = w @ V[:, None], w @ V[:, None].abs()
+        # An exponent of 2 (a score times log2 e) has up to four roundings of two products and three factors, relative to a magnitude of `most`, and
+        # so has the reference that is taken off it; the exponential two steps. A sum is taken by 16 positions, whose products may be cut off where they are added, a
+        # whole step twice, and 20 steps where partial sums are put together and divided; the pieces of a number leave out half a step each.
+        most = float((q.abs() @ K[:, None].abs().transpose(-1, -2) / math.sqrt(D)).amax())
+        t = size * U * (2 * 4 * most + 4 + 4 * (L / 16 + 1) + 20 + 6)
+        if c.dt == torch.bfloat16:
+            t = t + 1.1 * U16 * (o.abs() + size)             # as the documentation has it: probabilities may be rounded to bf16, the result is
+        got = out[r0:r0 + n].double().reshape(n, KH, H // KH, D).permute(1, 2, 0, 3)
+        worst = max(worst, float(((got - o).abs() / t).max()))
+        r0 += n
+    return worst
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,batch,length", [(1, 1, 1700), (1, 600, 200), (3, 2, 1700), (40, 2, 1700), (1, 3, 15)])
+def test_small_weights_count(api, ops, cache, rows, hd, new, batch, length):
+    """One key far above the rest: what the rest add up to is as exact as if they stood alone (a first position that takes most of the weight and
+    brings next to nothing is what trained models have)."""
+    c = Case(api, [new] * batch, [length] * batch, 4, 2, hd, cache, rows, k_scale=1.0, v_scale=1.0)
+    for above in (0, 13, 20, 27, 40):
+        first_key_takes_all(c, above)
+        c.describe()
+        worst = small_weights(c, attend(ops, c))
+        assert worst <= 1, f"{worst:.3g} of the bound, a key 2^{above} above the rest"
+    ops.status()
