@@ -303,7 +303,7 @@ int mlb_ops_status(mlb_ops* o, void* stream);
  *   fp4_e2m1: codes [num_pages][kv_heads][16][head_dim / 2] bytes (the even dim in the low half) and e4m3 scales
  *   [num_pages][kv_heads][16][head_dim / 16]; a value is code * scale * k_scale (or v_scale: one positive factor per
  *   pool, so that the scales of its blocks lie well inside e4m3's range; 1 where nothing is known).
- * head_dim 64 or 128, kv_heads up to 65535. page_table [batch][pt_stride]; entries behind a sequence's last page are not read. */
+ * head_dim 64 or 128, kv_heads up to 65535; of a bfloat16 pool num_pages * kv_heads * 16 below 2^31 where bfloat16 rows bring prompts. page_table [batch][pt_stride]; entries behind a sequence's last page are not read. */
 typedef struct mlb_paged_kv {
     void *kpool, *vpool;
     void *kscale, *vscale;   /* fp4_e2m1 only, else ignored                                 */

@@ -465,6 +465,10 @@ extern "C" int mlb_op_attn_paged(mlb_ops* o, const mlb_paged_kv* kv, const mlb_n
     if ((rc = check_rows("paged attention", "q", q, q_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
     if ((rc = check_rows("paged attention", "out", out, out_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
     if (gate_or_null && reinterpret_cast<uintptr_t>(gate_or_null) % 4) return fail(MLB_E_INVALID, "paged attention: gate is not on its type's boundary");
+    // prompts: a row of a bf16 pool is a coordinate of a tensor map, a 31-bit number
+    if (kv->dtype == MLB_DT_BF16 && row_dtype == MLB_DT_BF16 && paged_prompts(rows->row_start, rows->rows, rows->max_rows, heads / kv->kv_heads) &&
+        (long long)kv->num_pages * kv->kv_heads > 0x7fffffffLL / kKvBlock)
+        return fail(MLB_E_UNSUPPORTED, "paged attention: prompts over bfloat16 pages take pools of less than 2^31 rows of a head");
     if ((rc = check_count("paged attention", o, rows, heads, kv->head_dim))) return rc;
     if (rows->rows > 0 && q == out) return fail(MLB_E_INVALID, "paged attention: out may not be q");
     if (rows->rows == 0) return MLB_OK;

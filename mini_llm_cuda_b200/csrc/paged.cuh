@@ -170,6 +170,14 @@ __device__ __forceinline__ bool paged_sees(const AttnPagedParams& p, int pos, in
     return key <= pos && (p.window <= 0 || key > pos - p.window || key < p.sinks);
 }
 
+// Sequences of up to this many (token, head) rows per K/V head are taken page by page (paged_attn.cu), longer ones in tiles.
+constexpr int kSplitRows = 32;
+// Whether a call may bring a longer one
+inline bool paged_prompts(const int* row_start, int rows, int max_rows, int group) {
+    const long long most = max_rows > 0 && max_rows < rows ? max_rows : rows;
+    return row_start && most * group > kSplitRows;
+}
+
 cudaError_t attn_paged_launch(const AttnPagedParams& p, int dtype, int row_dtype, int head_dim, int sm_count, cudaStream_t st);
 size_t attn_paged_part_bytes(int sm_count);
 

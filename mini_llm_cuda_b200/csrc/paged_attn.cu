@@ -1041,11 +1041,15 @@ cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) 
     using S = SplitShape<KVT, RT, HD>;
     // Each warp alone where there are sequences and heads enough to give most of them whole items: nothing to put together in a CTA.
     const long long items = (long long)p.r.batch * p.c.kv_heads;
-    cudaError_t e = items >= 4LL * sm_count ? split_launch<KVT, RT, HD, 1>(p, sm_count, st) : split_launch<KVT, RT, HD, kSplitWarps>(p, sm_count, st);
-    if (e != cudaSuccess || !p.r.row_start) return e;
-    const long long most = p.r.max_rows > 0 ? std::min(p.r.max_rows, p.r.rows) : p.r.rows;
-    if (most * p.group <= kSplitRows) return e;
-    if constexpr (sizeof(KVT) <= 2 && sizeof(RT) == 2) return attn_prompt_launch(p, sizeof(KVT) == 1 ? MLB_DT_FP4_E2M1 : MLB_DT_BF16, HD, st);
+    const bool prompts = paged_prompts(p.r.row_start, p.r.rows, p.r.max_rows, p.group);
+    constexpr bool TILES = sizeof(KVT) <= 2 && sizeof(RT) == 2;
+    constexpr int dtype = sizeof(KVT) == 1 ? MLB_DT_FP4_E2M1 : MLB_DT_BF16;
+    PromptMaps maps;
+    cudaError_t e = TILES && prompts ? attn_prompt_maps(p, dtype, HD, &maps) : cudaSuccess;
+    if (e != cudaSuccess) return e;
+    e = items >= 4LL * sm_count ? split_launch<KVT, RT, HD, 1>(p, sm_count, st) : split_launch<KVT, RT, HD, kSplitWarps>(p, sm_count, st);
+    if (e != cudaSuccess || !prompts) return e;
+    if constexpr (TILES) return attn_prompt_launch(p, dtype, HD, maps, st);
     const size_t smem = (size_t)S::QWORDS * 8 + split_ring_bytes<KVT, HD, kSplitWarps>();
     e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e != cudaSuccess) return e;

@@ -701,29 +701,30 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
 }
 
 template <typename KVT, int HD>
-cudaError_t launch(EncodeTiledFn enc, const AttnPagedParams& p, cudaStream_t st) {
-    alignas(64) CUtensorMap tk, tv;
-    std::memset(&tk, 0, sizeof tk);
-    std::memset(&tv, 0, sizeof tv);
-    const uint64_t rows = (uint64_t)p.c.num_pages * p.c.kv_heads * kKvBlock;
-    if (rows > 0x7fffffffu) return cudaErrorInvalidValue;        // (a row's coordinate is a 31-bit number; such a pool would not fit the device)
-    if (sizeof(KVT) == 2 && (make_bf16_map(enc, &tk, p.c.kpool, rows, HD, kKvBlock) || make_bf16_map(enc, &tv, p.c.vpool, rows, HD, kKvBlock)))
-        return cudaErrorInvalidValue;
+cudaError_t launch(const AttnPagedParams& p, const PromptMaps& maps, cudaStream_t st) {
     const size_t smem = PromptSmem<HD, kPpTiles<KVT>, kPpEarly<KVT, HD>>::total + 1024;
     cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<KVT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.r.rows * p.group / (128 * kPpTiles<KVT>) + p.r.batch;
     // It starts while the kernels of the short sequences, which it shares nothing with, are at work.
-    return launch_after(attn_prompt_kernel<KVT, HD>, dim3((unsigned)(tiles * p.c.kv_heads)), kPpThreads<KVT>, smem, st, tk, tv, p);
+    return launch_after(attn_prompt_kernel<KVT, HD>, dim3((unsigned)(tiles * p.c.kv_heads)), kPpThreads<KVT>, smem, st, maps.k, maps.v, p);
 }
 
 }  // namespace
 
-cudaError_t attn_prompt_launch(const AttnPagedParams& p, int dtype, int head_dim, cudaStream_t st) {
+cudaError_t attn_prompt_maps(const AttnPagedParams& p, int dtype, int head_dim, PromptMaps* maps) {
+    std::memset(maps, 0, sizeof *maps);
+    if (dtype != MLB_DT_BF16) return cudaSuccess;
     static const EncodeTiledFn enc = get_encode_tiled();
     if (!enc) return cudaErrorNotSupported;
-    if (dtype == MLB_DT_FP4_E2M1) return head_dim == 64 ? launch<fp4_t, 64>(enc, p, st) : launch<fp4_t, 128>(enc, p, st);
-    return head_dim == 64 ? launch<bf16_t, 64>(enc, p, st) : launch<bf16_t, 128>(enc, p, st);
+    const uint64_t rows = (uint64_t)p.c.num_pages * p.c.kv_heads * kKvBlock;
+    if (make_bf16_map(enc, &maps->k, p.c.kpool, rows, head_dim, kKvBlock) || make_bf16_map(enc, &maps->v, p.c.vpool, rows, head_dim, kKvBlock)) return cudaErrorInvalidValue;
+    return cudaSuccess;
+}
+
+cudaError_t attn_prompt_launch(const AttnPagedParams& p, int dtype, int head_dim, const PromptMaps& maps, cudaStream_t st) {
+    if (dtype == MLB_DT_FP4_E2M1) return head_dim == 64 ? launch<fp4_t, 64>(p, maps, st) : launch<fp4_t, 128>(p, maps, st);
+    return head_dim == 64 ? launch<bf16_t, 64>(p, maps, st) : launch<bf16_t, 128>(p, maps, st);
 }
 
 }  // namespace mlb

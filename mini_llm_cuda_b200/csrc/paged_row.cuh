@@ -106,7 +106,4 @@ static cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Sequences of up to this many (token, head) rows per K/V head are taken page by page (paged_attn.cu), longer ones in tiles.
-constexpr int kSplitRows = 32;
-
 }  // namespace mlb

@@ -83,3 +83,22 @@ def test_small_weights_count(api, ops, cache, rows, hd, new, batch, length):
         worst = small_weights(c, attend(ops, c))
         assert worst <= 1, f"{worst:.3g} of the bound, a key 2^{above} above the rest"
     ops.status()
+
+
+# ---- pools of more than 2^31 rows --------------------------------------------------------------------------------------
+def test_4_bit_pools_may_have_more_rows(api, ops):
+    """2^31 rows of a head fit the device at 4 bits. The pool described here is that large, the one behind it holds the pages that the table names."""
+    import torch
+    c = Case(api, [1, 90], [300, 120], 2, 1, 64, "fp4", "bf16")
+    c.kv.struct.num_pages = (1 << 27) + 1
+    want, tol = c.attention(50, 3)
+    out = attend(ops, c, 50, 3)
+    ops.status()
+    assert float(((out.double() - want).abs() - tol).max()) <= 0
+    # of bf16 it is refused where prompts may come, before anything is written
+    c = Case(api, [1, 90], [300, 120], 2, 1, 64, "bf16", "bf16")
+    c.kv.struct.num_pages = (1 << 27) + 1
+    out = torch.full_like(c.q, 777.0)
+    with pytest.raises(api.MlbError, match="2\\^31"):
+        attend(ops, c, 50, 3, out=out)
+    assert bool((out == 777.0).all())

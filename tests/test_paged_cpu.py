@@ -125,3 +125,18 @@ def test_refused_head_counts(api):
     L, kv, rows, p = api.lib(), cache(api), new_rows(api), 1 << 20
     assert L.mlb_op_kv_append(None, C.byref(kv), C.byref(rows), api.DT_BF16, p, 4096, p, 4096, None, 0, p, 1 << 30, p, 1 << 30, 8 * 65535 + 1, None) \
         == api.MLB_E_UNSUPPORTED
+
+
+def test_refused_pools_of_too_many_rows(api):
+    """A row of a bf16 pool is a coordinate of a tensor map where prompts may come; pools of 4 bits and steps have no such limit."""
+    L, p = api.lib(), 1 << 20
+
+    def status(dtype=api.DT_BF16, row_start=64, max_rows=0, pages=(1 << 26) + 1, rows=200):
+        kv = cache(api, dtype=dtype, num_pages=pages, kscale=256, vscale=512)
+        nr = new_rows(api, row_start=row_start, rows=rows, max_rows=max_rows)
+        rc = L.mlb_op_attn_paged(None, C.byref(kv), C.byref(nr), api.DT_BF16, p, 4096, None, p, 4096, 4, 0.0, 0, 0, None)
+        return rc, b"2^31" in L.mlb_last_error()
+
+    assert status() == (api.MLB_E_UNSUPPORTED, True)
+    for kw in (dict(dtype=api.DT_FP4), dict(row_start=None), dict(max_rows=16), dict(rows=16), dict(pages=(1 << 26) - 1)):
+        assert status(**kw) == (api.MLB_E_INVALID, False)    # (no handle)
