@@ -95,11 +95,8 @@ __device__ __forceinline__ void e2m1x8_to_f16(uint32_t codes, uint32_t (&o)[4]) 
         : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
         : "r"(codes));
 }
-__device__ __forceinline__ float e2m1_value(int code) {
-    const int m = code & 7;
-    const float v = m < 2 ? 0.5f * (float)m : (1.f + 0.5f * (float)(m & 1)) * (float)(1 << ((m >> 1) - 1));
-    return code & 8 ? -v : v;
-}
+// Low four bits of `code`; its exponent and mantissa at the low end of a float's exponent are the value times 2^-126
+__device__ __forceinline__ float e2m1_value(uint32_t code) { return __uint_as_float((code & 8u) << 28 | (code & 7u) << 22) * 8.507059173023462e37f; }
 // Two e4m3 values -> two halves (exact)
 __device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t two) {
     uint32_t o;

@@ -682,11 +682,11 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
             const unsigned mine = __ballot_sync(0xffffffffu, odd && in && good);
             if (lane == 0) odd_rows[t][half][warp & 3] = mine;
             pair_sync();                                         // (what either warp has written is written)
-            if (half == 0) {
-                for (unsigned again = odd_rows[t][0][warp & 3] | odd_rows[t][HALVES - 1][warp & 3]; again; again &= again - 1) {
-                    const int src = __ffs(again) - 1;
-                    careful_row<KVT, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
-                }
+            // the pair's warps in turn
+            unsigned again = (odd_rows[t][0][warp & 3] | odd_rows[t][HALVES - 1][warp & 3]) & (HALVES == 1 ? 0xffffffffu : half ? 0xaaaaaaaau : 0x55555555u);
+            for (; again; again &= again - 1) {
+                const int src = __ffs(again) - 1;
+                careful_row<KVT, bf16_t, HD>(p, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, row, src), __shfl_sync(0xffffffffu, h, src));
             }
         }
         tc_fence_before();

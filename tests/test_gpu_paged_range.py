@@ -1,4 +1,4 @@
-"""GPU: paged attention where a few numbers decide the answer: weights over a wide range, every position by itself, positions that hold no numbers."""
+"""GPU: paged operators at the ends of their ranges: weights over a wide range, pools of many rows, values that are no numbers."""
 import math
 
 import numpy as np
@@ -102,3 +102,69 @@ def test_4_bit_pools_may_have_more_rows(api, ops):
     with pytest.raises(api.MlbError, match="2\\^31"):
         attend(ops, c, 50, 3, out=out)
     assert bool((out == 777.0).all())
+
+
+# ---- values that are no numbers ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("heads,hd", [(2, 64), (8, 128)])
+@pytest.mark.parametrize("new,length", [(1, 300), (3, 77), (50, 90)])
+def test_one_value_is_no_number(api, ops, cache, rows, heads, hd, new, length):
+    """An infinite value in one dim of one position (4 bits: a NaN scale, sixteen dims): the other dims, and rows that do not see the position, are as
+    if it were not there, and those that see it get no number in that dim."""
+    import torch
+    c = Case(api, [new], [length], heads, 2, hd, cache, rows)
+    for at in (length - new + new // 2, 20):
+        page, slot = int(c.table[0, at // 16]), at % 16
+        if cache == "fp4":
+            before = c.vscale.view(torch.uint8)[page, 1, slot, 2].clone()
+            c.vscale.view(torch.uint8)[page, 1, slot, 2] = 0x7f
+            dims = range(32, 48)
+        else:
+            before = c.vpool[page, 1, slot, 33].clone()
+            c.vpool[page, 1, slot, 33] = math.inf
+            dims = range(33, 34)
+        want, tol = c.attention()
+        out = attend(ops, c).double().reshape(new, 2, heads // 2, hd)
+        sees = torch.arange(length - new, length, device="cuda") >= at
+        hit = torch.zeros(new, 2, heads // 2, hd, dtype=torch.bool, device="cuda")
+        hit[:, 1, :, dims.start:dims.stop] = sees[:, None, None]
+        assert not bool(torch.isfinite(out[hit]).any())
+        if cache != "fp4":
+            assert bool((out[hit] == math.inf).all())
+        over = (out - want.reshape(out.shape)).abs() - tol.reshape(out.shape)
+        assert float(over[~hit].max()) <= 0
+        if cache == "fp4":
+            c.vscale.view(torch.uint8)[page, 1, slot, 2] = before
+        else:
+            c.vpool[page, 1, slot, 33] = before
+    ops.status()
+
+
+@pytest.mark.parametrize("cache,rows", [("bf16", "bf16"), ("f32", "f32"), ("fp4", "bf16"), ("fp4", "f32")])
+@pytest.mark.parametrize("new,length", [(1, 20000), (1000, 1000)])
+def test_a_row_without_an_answer_ends_early(api, ops, cache, rows, new, length):
+    """A NaN among the first keys: nothing that follows can make the rows numbers, so they do not cost what a row done by hand does (over 300 times the
+    call for these sizes, and 1 to 5 times where it ends with the answer)."""
+    import torch
+
+    def best():
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = attend(ops, c)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times), out
+
+    c = Case(api, [new], [length], 16, 4, 128, cache, rows)
+    clean, _ = best()
+    page = int(c.table[0, 0])
+    if cache == "fp4":
+        c.kscale.view(torch.uint8)[page, :, 3, 0] = 0x7f
+    else:
+        c.kpool[page, :, 3, 7] = math.nan
+    bad, out = best()
+    assert bool(torch.isnan(out[max(0, 3 - (length - new)):]).all()) and bool(torch.isfinite(out[:max(0, 3 - (length - new))]).all())
+    assert bad < 40 * clean, (bad, clean)
