@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import sys
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -489,8 +490,9 @@ class NewRows:
 
 class Ops:
     """Operators over paged caches on one device and stream (mlb_ops). Row tensors are [rows][heads * head_dim] (or
-    [rows][heads][head_dim]) fp32 or bf16 with any stride between rows; `stream` is a CUDA stream's handle (0: the default
-    stream). Calls do not wait for the stream; status() does, and raises for what the kernels found wrong with the data."""
+    [rows][heads][head_dim]) fp32 or bf16 with any stride between rows; `stream` is a CUDA stream's handle (None: torch's current
+    stream of the device, 0: the default stream). Calls do not wait for the stream; status() does, and raises for what the kernels
+    found wrong with the data."""
 
     def __init__(self, device: int = 0):
         self._h = C.c_void_p()
@@ -525,7 +527,10 @@ class Ops:
             raise ValueError(f"{what} is {x.dtype}: expected float32 or bfloat16")
         return dt
 
-    def kv_append(self, cache: PagedKV, rows: NewRows, k, v, rope=None, q=None, q_out=None, heads: int = 0, stream: int = 0):
+    def _stream(self) -> int:
+        return sys.modules["torch"].cuda.current_stream(self.device).cuda_stream         # (the tensors come from there)
+
+    def kv_append(self, cache: PagedKV, rows: NewRows, k, v, rope=None, q=None, q_out=None, heads: int = 0, stream: Optional[int] = None):
         """Rotates k (and q into q_out, which may be q) by the rows' positions and writes k and v to their pages."""
         dtype, shape = k.dtype, (rows.rows, cache.width)
         dt = self._check(cache, rows, k, "k")
@@ -548,22 +553,22 @@ class Ops:
                     not rope.is_contiguous() or rope.get_device() != self.device:
                 raise ValueError(f"rope must be a contiguous fp32 [positions][{cache.head_dim}] on CUDA device {self.device}")
             rp, rl = rope.data_ptr(), shape[0]
-        rc = self._append(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, rp, rl, qp, qs, op, os_, heads, stream)
+        rc = self._append(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, rp, rl, qp, qs, op, os_, heads, self._stream() if stream is None else stream)
         if rc:
             check(rc)
 
-    def kv_read(self, cache: PagedKV, rows: NewRows, k_out, v_out, stream: int = 0):
+    def kv_read(self, cache: PagedKV, rows: NewRows, k_out, v_out, stream: Optional[int] = None):
         """The rows' cached keys and values, as values."""
         dtype, shape = k_out.dtype, (rows.rows, cache.width)
         dt = self._check(cache, rows, k_out, "k_out")
         kp, ks = self._rows(k_out, "k_out", shape, dtype)
         vp_, vs = self._rows(v_out, "v_out", shape, dtype)
-        rc = self._read(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, stream)
+        rc = self._read(self._h, cache.ref, rows.ref, dt, kp, ks, vp_, vs, self._stream() if stream is None else stream)
         if rc:
             check(rc)
 
     def attn_paged(self, cache: PagedKV, rows: NewRows, q, out, heads: int, gate=None, scale: float = 0.0, window: int = 0, sinks: int = 0,
-                   stream: int = 0):
+                   stream: Optional[int] = None):
         """Causal attention of the rows, optionally within a window and to the first `sinks` positions (mlb_op_attn_paged)."""
         dtype, shape = q.dtype, (rows.rows, heads * cache.head_dim)
         dt = self._check(cache, rows, q, "q")
@@ -574,12 +579,14 @@ class Ops:
             if _row_dtype(gate.dtype) != DT_F32 or not gate.is_contiguous():
                 raise ValueError("gate must be a contiguous fp32 tensor")
             gp, _ = self._rows(gate, "gate", shape, gate.dtype)
-        rc = self._attn(self._h, cache.ref, rows.ref, dt, qp, qs, gp, op, os_, heads, scale, window, sinks, stream)
+        rc = self._attn(self._h, cache.ref, rows.ref, dt, qp, qs, gp, op, os_, heads, scale, window, sinks, self._stream() if stream is None else stream)
         if rc:
             check(rc)
 
-    def status(self, stream: int = 0):
+    def status(self, stream: Optional[int] = None):
         """Waits for the stream; raises if a call since the last status() met a bad page id, row range or length."""
+        if stream is None:
+            stream = self._stream() if "torch" in sys.modules else 0
         check(lib().mlb_ops_status(self._h, stream))
 
     def close(self):

@@ -140,3 +140,51 @@ def test_refused_pools_of_too_many_rows(api):
     assert status() == (api.MLB_E_UNSUPPORTED, True)
     for kw in (dict(dtype=api.DT_FP4), dict(row_start=None), dict(max_rows=16), dict(rows=16), dict(pages=(1 << 26) - 1)):
         assert status(**kw) == (api.MLB_E_INVALID, False)    # (no handle)
+
+
+class FakeTensor:
+    """As much of a CUDA tensor as the calls look at."""
+
+    def __init__(self, dtype, rows, width):
+        import torch
+        self.dtype, self.shape, self._stride = dtype, torch.Size((rows, width)), (width, 1)
+
+    def get_device(self):
+        return 0
+
+    def stride(self, i=None):
+        return self._stride if i is None else self._stride[i]
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+@pytest.fixture
+def fake_ops(api, monkeypatch):
+    """api.Ops whose calls end in a list instead of the library, on a device whose current torch stream is 4711."""
+    import types
+    import torch
+    ops, calls = api.Ops.__new__(api.Ops), []
+    ops._h, ops.device = C.c_void_p(), 0
+    ops._append = ops._read = ops._attn = lambda *a: calls.append(a) or 0
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=4711) if device == 0 else None)
+    cache = types.SimpleNamespace(batch=3, device=0, width=128, head_dim=64, ref=None)
+    rows = types.SimpleNamespace(batch=3, device=0, rows=5, ref=None)
+    return ops, calls, cache, rows
+
+
+def test_torch_current_stream_unless_told(api, fake_ops, monkeypatch):
+    """A call without a stream runs behind what torch has on its current one."""
+    import types
+    import torch
+    ops, calls, cache, rows = fake_ops
+    x, y = FakeTensor(torch.bfloat16, 5, 128), FakeTensor(torch.bfloat16, 5, 256)
+    fake = types.SimpleNamespace(mlb_ops_status=lambda h, stream: calls.append((stream,)) or 0)
+    monkeypatch.setattr(api, "lib", lambda: fake)
+    for kw, want in ((dict(), 4711), (dict(stream=0), 0), (dict(stream=5), 5)):
+        ops.kv_append(cache, rows, x, x, **kw)
+        ops.kv_read(cache, rows, x, x, **kw)
+        ops.attn_paged(cache, rows, y, y, heads=4, **kw)
+        ops.status(*kw.values())
+        assert [c[-1] for c in calls] == [want] * 4
+        calls.clear()
