@@ -328,7 +328,7 @@ typedef struct mlb_new_rows {
 /* Writes k and v [rows][kv_heads * head_dim] (row_dtype float32 or bfloat16; strides in elements from row to row) to
  * the pages of their positions. With a table rope [rope_len][head_dim] of interleaved (cos, sin) as mlb_rope_table makes
  * it, dims 2i and 2i + 1 of k are turned by the table row of the position first; so is q [rows][heads * head_dim], where
- * given, into q_out (which may be q, but not overlap it otherwise). Each product and sum of the rotation is one fp32 operation. In a 4-bit cache 16 dims
+ * given, into q_out (which may be q, with its stride, but not overlap it otherwise). Each product and sum of the rotation is one fp32 operation. In a 4-bit cache 16 dims
  * get the scale e4m3(max|x| / (6 k_scale)) and the codes nearest to x * (1 / (scale * k_scale)), ties to the even code; an
  * infinity takes the largest code and scale, a NaN is stored as some number. Two sequences must not append to one page. */
 int mlb_op_kv_append(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows, int row_dtype, const void* k,

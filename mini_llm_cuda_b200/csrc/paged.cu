@@ -413,6 +413,8 @@ extern "C" int mlb_op_kv_append(mlb_ops* o, const mlb_paged_kv* kv, const mlb_ne
         if ((rc = check_rows("append", "q", q_or_null, q_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
         if ((rc = check_rows("append", "q_out", q_out, q_out_stride, (int64_t)heads * kv->head_dim, row_dtype, rows->rows))) return rc;
     }
+    if (q_or_null && q_or_null == q_out && q_stride != q_out_stride && rows->rows > 1)
+        return fail(MLB_E_INVALID, "append: q_out may be q with the same stride, and not overlap it otherwise");
     if ((rc = check_count("append", o, rows, 2LL * kv->kv_heads + (q_or_null ? heads : 0), kv->head_dim))) return rc;
     if (rows->rows == 0) return MLB_OK;
     const int elt = row_dtype == MLB_DT_F32 ? 4 : 2;

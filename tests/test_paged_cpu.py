@@ -188,3 +188,16 @@ def test_torch_current_stream_unless_told(api, fake_ops, monkeypatch):
         ops.status(*kw.values())
         assert [c[-1] for c in calls] == [want] * 4
         calls.clear()
+
+
+def test_refused_rotation_in_place_with_another_stride(api):
+    """Row i of q_out over row j of q: rotated and not rotated rows in each other's place."""
+    L, kv, rows, p = api.lib(), cache(api), new_rows(api), 1 << 20
+
+    def status(q_stride, out_stride, rows=rows):
+        rc = L.mlb_op_kv_append(None, C.byref(kv), C.byref(rows), api.DT_BF16, p, 4096, p, 4096, None, 0, p, q_stride, p, out_stride, 4, None)
+        return rc, b"same stride" in L.mlb_last_error()
+
+    assert status(4096, 512) == (api.MLB_E_INVALID, True)
+    assert status(4096, 4096) == (api.MLB_E_INVALID, False)              # (no handle)
+    assert status(4096, 512, new_rows(api, batch=1, rows=1)) == (api.MLB_E_INVALID, False)
