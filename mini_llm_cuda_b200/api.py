@@ -418,6 +418,7 @@ _CACHE_DTYPES = {**_ROW_DTYPES, "torch.uint8": DT_FP4}
 
 
 _dtype_seen = {}
+_INT32_MAX = (1 << 31) - 1              # (ctypes takes the low 32 bits of a larger number without a word)
 
 
 def _row_dtype(dtype):
@@ -484,7 +485,7 @@ class NewRows:
             _dense(row_start, "row_start", ("torch.int32",), (self.batch + 1,))
         self.tensors = [t for t in (kv_lens, row_start) if t is not None]
         self.device = _one_device(self.tensors)
-        self.struct = NewRowsStruct(row_start.data_ptr() if row_start is not None else None, kv_lens.data_ptr(), self.batch, self.rows, max_rows)
+        self.struct = NewRowsStruct(row_start.data_ptr() if row_start is not None else None, kv_lens.data_ptr(), self.batch, self.rows, min(max_rows, _INT32_MAX))
         self.ref = C.byref(self.struct)
 
 
@@ -570,6 +571,8 @@ class Ops:
     def attn_paged(self, cache: PagedKV, rows: NewRows, q, out, heads: int, gate=None, scale: float = 0.0, window: int = 0, sinks: int = 0,
                    stream: Optional[int] = None):
         """Causal attention of the rows, optionally within a window and to the first `sinks` positions (mlb_op_attn_paged)."""
+        if not (0 <= window <= _INT32_MAX and 0 <= sinks <= _INT32_MAX):         # beyond every position; the call refuses what is negative
+            window, sinks = (max(-1, min(x, _INT32_MAX)) for x in (window, sinks))
         dtype, shape = q.dtype, (rows.rows, heads * cache.head_dim)
         dt = self._check(cache, rows, q, "q")
         qp, qs = self._rows(q, "q", shape, dtype)

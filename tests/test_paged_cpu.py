@@ -201,3 +201,18 @@ def test_refused_rotation_in_place_with_another_stride(api):
     assert status(4096, 512) == (api.MLB_E_INVALID, True)
     assert status(4096, 4096) == (api.MLB_E_INVALID, False)              # (no handle)
     assert status(4096, 512, new_rows(api, batch=1, rows=1)) == (api.MLB_E_INVALID, False)
+
+
+def test_numbers_beyond_32_bits(api, fake_ops):
+    """A window, a count of first positions or a most of rows above 2^31 is one that nothing reaches, and not its low 32 bits."""
+    import torch
+    ops, calls, cache, rows = fake_ops
+    y = FakeTensor(torch.bfloat16, 5, 256)
+    top = (1 << 31) - 1
+    for window, sinks, want in ((5, 3, (5, 3)), ((1 << 32) + 5, 1 << 32, (top, top)), (top + 1, 0, (top, 0)), (-(1 << 32), 4, (-1, 4)), (0, -(1 << 33) - 7, (0, -1))):
+        ops.attn_paged(cache, rows, y, y, heads=4, window=window, sinks=sinks)
+        assert calls.pop()[-3:-1] == want
+    lens = FakeTensor(torch.int32, 1, 3)
+    lens.is_cuda, lens.is_contiguous, lens.numel = True, lambda: True, lambda: 3
+    assert api.NewRows(lens, 3, max_rows=(1 << 32) + 1).struct.max_rows == top
+    assert api.NewRows(lens, 3, max_rows=7).struct.max_rows == 7
