@@ -168,3 +168,155 @@ def test_a_row_without_an_answer_ends_early(api, ops, cache, rows, new, length):
     bad, out = best()
     assert bool(torch.isnan(out[max(0, 3 - (length - new)):]).all()) and bool(torch.isfinite(out[:max(0, 3 - (length - new))]).all())
     assert bad < 40 * clean, (bad, clean)
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_hidden_scales_hold_no_numbers(api, ops, rows, new):
+    """4 bits: NaN scales at positions that no row sees, as unused slots of a fresh page may have them."""
+    import torch
+    lens = [new + 200, new + 37, new, new + 129]
+    window, sinks = 20, 5
+    c = Case(api, [new] * 4, lens, 8, 2, 128, "fp4", rows)
+    want, tol = c.attention(window, sinks)
+    hidden = torch.ones(c.n_pages, 16, dtype=torch.bool, device="cuda")
+    for b, L in enumerate(lens):
+        for j in range(L):
+            if j < sinks or j > L - new - window:
+                hidden[int(c.table[b, j // 16]), j % 16] = False
+    bad = torch.tensor([0x7f, 0xff], dtype=torch.uint8, device="cuda")
+    for n, scale in enumerate((c.kscale, c.vscale)):
+        v = scale.view(torch.uint8).permute(0, 2, 1, 3)
+        v[hidden] = bad[(torch.arange(int(hidden.sum()), device="cuda") + n) % 2][:, None, None].expand(-1, c.kv_heads, 8)
+    out = attend(ops, c, window, sinks).double()
+    assert bool(torch.isfinite(out).all())
+    assert float(((out - want).abs() - tol).max()) <= 0
+    ops.status()
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,hd", [(2, 64), (8, 128)])
+@pytest.mark.parametrize("new,length", [(3, 60), (40, 60), (200, 260)])
+def test_a_later_row_sees_no_scale(api, ops, rows, heads, hd, new, length):
+    """4 bits: a position with NaN scales that later rows see and earlier ones do not."""
+    import torch
+    c = Case(api, [new], [length], heads, 2, hd, "fp4", rows)
+    want, tol = c.attention()
+    at = length - new // 2 - 1
+    page, slot, before = int(c.table[0, at // 16]), at % 16, at - (length - new)
+    for scale in (c.vscale, c.kscale):
+        scale.view(torch.uint8)[page, :, slot] = 0xff
+        out = attend(ops, c).double()
+        assert float(((out - want).abs() - tol)[:before].max()) <= 0
+        assert bool(torch.isnan(out[before:]).all())
+
+
+def test_4_bit_offsets_past_32_bits(api, ops):
+    """Codes more than 2^32 bytes from the pool's start: appended, read and attended to as in a small pool."""
+    import torch
+    kv_heads, hd = 8, 128
+    pages = ((1 << 32) + (1 << 27)) // (kv_heads * 16 * hd // 2)
+    if torch.cuda.mem_get_info()[0] < 3 * pages * kv_heads * 16 * hd:
+        pytest.skip("not enough device memory")
+    small, large = (Case(api, [1, 150], [400, 170], 16, kv_heads, hd, "fp4", "bf16", seed=9) for _ in range(2))
+    n = small.n_pages
+    names = ["kpool", "vpool", "kscale", "vscale"]
+    for name in names:
+        x = getattr(large, name)
+        big = torch.zeros((pages, *x.shape[1:]), dtype=torch.uint8, device="cuda")
+        big[pages - n:].copy_(x.view(torch.uint8))
+        setattr(large, name, big if name.endswith("pool") else big.view(x.dtype))
+    large.table += pages - n
+    large.describe()
+    read = []
+    for c in (small, large):
+        out = attend(ops, c, 100, 3)
+        ops.kv_append(c.kv, c.nr, c.k, c.v)
+        ko, vo = torch.empty_like(c.k), torch.empty_like(c.v)
+        ops.kv_read(c.kv, c.nr, ko, vo)
+        read.append((out, ko, vo))
+    ops.status()
+    for x, y in zip(*read):
+        assert bool((x == y).all())
+    for name in names:
+        x, y = (getattr(c, name).view(torch.uint8) for c in (small, large))
+        assert bool((x == y[pages - n:]).all()) and not bool(y[:pages - n].any())
+
+
+# ---- every position once -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd", [(8, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("kind", ["one", "few", "many", "crowd", "rows", "prompts"])
+def test_every_position_counts_once(api, ops, cache, rows, heads, kv_heads, hd, kind):
+    """Queries of zeros weigh all that is visible alike. Values count: one dim holds ones at every hd-th position (or page), the next dim at the ones after
+    them, so that a position or page left out or taken twice, at any share's, tile's or page's border, is off by a whole number."""
+    import torch
+    rng = np.random.default_rng(11)
+    new, lens, ragged = {
+        "one": ([1], [5003], False),
+        "few": ([1] * 9, [3333, 1, 16, 2049, 700, 17, 4096, 31, 1200], False),
+        "many": ([1] * 70, rng.integers(1, 1500, size=70).tolist(), False),
+        "crowd": ([1] * 640, rng.integers(1, 300, size=640).tolist(), False),
+        "rows": ([1, 3, 0, 4, 2, 8, 1], [2222, 1003, 5, 64, 18, 3000, 1], True),
+        "prompts": ([130, 1, 33, 257, 64], [900, 40, 1033, 257, 2000], True),
+    }[kind]
+    c = Case(api, new, lens, heads, kv_heads, hd, cache, rows, ragged=ragged, k_scale=1.0, v_scale=1.0)
+    c.q.zero_()
+    if cache == "fp4":
+        c.vscale.copy_(torch.ones(c.vscale.shape, device="cuda"))
+    t = torch.arange(max(lens), device="cuda")
+    for which in (t % hd, t // 16 % hd):
+        c.vpool.zero_()
+        ones = (which[:, None] == torch.arange(hd, device="cuda")).double()
+        for b, L in enumerate(lens):
+            v = ones[:L]
+            if cache == "fp4":
+                v = (v[:, 0::2] * 2 + v[:, 1::2] * 32).to(torch.uint8)               # code 2 is 1
+            full = torch.zeros((L + 15) // 16 * 16, v.shape[1], dtype=c.vpool.dtype, device="cuda")
+            full[:L] = v.to(c.vpool.dtype)
+            c.vpool[c.table[b, :(L + 15) // 16].long()] = full.reshape(-1, 1, 16, v.shape[1])
+        for window, sinks in ((0, 0), (1000, 37), (77, 3)):
+            out = attend(ops, c, window, sinks).double().reshape(c.rows, heads, hd)
+            r0 = 0
+            for n, L in zip(new, lens):
+                p = torch.arange(L - n, L, device="cuda")[:, None]
+                sees = t[None, :L] <= p
+                if window:
+                    sees &= (t[None, :L] > p - window) | (t[None, :L] < sinks)
+                count, total = sees.double() @ ones[:L], sees.sum(1).double()
+                off = (out[r0:r0 + n] * total[:, None, None] - count[:, None]).abs()
+                # equal weights are whole powers of two and sums of ones exact: the answer is rounded once or twice, and so off by less than a half
+                assert n == 0 or float(off.max()) < 0.5, (kind, n, L, window, float(off.max()))
+                r0 += n
+    ops.status()
+
+
+@pytest.mark.parametrize("cache", ["f32", "bf16", "fp4"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,batch,length", [(1, 1, 2900), (1, 600, 130), (4, 3, 700), (70, 2, 700)])
+def test_fp32_rows_to_fp32(api, ops, cache, hd, new, batch, length):
+    """fp32 rows, relative to the sum of w |v| of each number: an operand rounded to bf16 on the way would show (some 2^-9 of a score of 3, which the sum over
+    some hundred positions leaves a tenth of)."""
+    import torch
+    c = Case(api, [new] * batch, [length] * batch, 4, 2, hd, cache, "f32")
+    if cache == "fp4":                               # values of about the size of the others'
+        c.k_scale, c.v_scale = 0.02, 0.02
+        c.describe()
+    out = attend(ops, c, length // 2, 3)
+    KH, G, r0 = c.kv_heads, c.heads // c.kv_heads, 0
+    for b, (n, L) in enumerate(zip(c.new, c.lens)):
+        q = c.q[r0:r0 + n].double().reshape(n, KH, G, hd).permute(1, 2, 0, 3)
+        K, V = c.cached("k", b, L), c.cached("v", b, L)
+        p, j = torch.arange(L - n, L, device="cuda")[:, None], torch.arange(L, device="cuda")[None]
+        s = (q @ K[:, None].transpose(-1, -2) / math.sqrt(hd)).masked_fill((j > p) | (j <= p - length // 2) & (j >= 3), -math.inf)
+        w = torch.softmax(s, dim=-1)
+        o, size = w @ V[:, None], w @ V[:, None].abs()
+        most = (q.abs() @ K[:, None].abs().transpose(-1, -2) / math.sqrt(hd)).amax(-1, keepdim=True)
+        # A score is taken in hd / 16 steps of up to six products of pieces, each of which may cut off where it adds (a whole step, 2 U, of at most `most`), has
+        # three factors, and 4-bit queries' 22 bits (4 U); so has the maximum that is taken off it. The sum over weights: L / 16 such steps. The exponential,
+        # the division and the joining of partial sums: 30.
+        t = size * U * (2 * (2 * 6 * (hd / 16) + 4 + 4) * most + 2 * 6 * (L / 16 + 1) + 30)
+        got = out[r0:r0 + n].double().reshape(n, KH, G, hd).permute(1, 2, 0, 3)
+        assert float(((got - o).abs() / t).max()) <= 1
+        r0 += n
+    ops.status()
