@@ -342,7 +342,7 @@ int mlb_op_kv_read(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows,
  * [rows][heads * head_dim] of row_dtype (out is not q), heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
  * (0: 1 / sqrt(head_dim)); gate (nullable) fp32 [rows][heads * head_dim] multiplies the output. Sums and softmax statistics are
  * fp32; with float32 rows so is everything else to fp32's own rounding (over 4-bit pages q is taken to 22 bits, and to no finer than 2^-33 of
- * its row's largest), with bfloat16 rows probabilities may be rounded to bf16: each of them, however small beside the largest. What
+ * its row's largest), with bfloat16 rows probabilities may be rounded to bf16: each of them, down to 2^-50 of the row's largest. What
  * lies at positions that a row does not see (numbers or not) does not reach its output. A row whose answer is no number, or that meets an infinity, is
  * done by one warp alone, some 0.15 us for each position that it sees (a prompt of 2000 with an infinite value near its start 6 ms instead of 0.06),
  * but no further than to where all of it is NaN. */

@@ -20,13 +20,12 @@ namespace {
 // 16-bit halves it pairs up with byte permutes. S lies with positions along the lanes and rows within them, as O does: a running maximum
 // and its rescaling need no exchange between lanes but the maximum itself, and that only when a score passes the old one by 2^8; P is
 // turned round by movmatrix.
-// fp32 numbers are taken in pieces whose products are exact: fp32 queries, K, V and probabilities in three bf16, probabilities of bf16 rows in two (4-bit pages: one). Products of
+// fp32 numbers are taken in pieces whose products are exact: fp32 queries, K, V and probabilities in three bf16, probabilities of bf16 rows in two. Products of
 // pieces below 2^-24 of the whole are left out. 4-bit codes times their e4m3 scale are exact halves, to which the conversion instruction brings them, and meet
 // queries as halves (fp32: two of them, bf16: one), the row scaled by a power of two to lie within their range.
-// Probabilities are in bf16 and not in halves over 4-bit pages too, where the codes of V are widened to bf16 for them: a probability may have any magnitude, and
-// where one position outweighs the rest and brings next to nothing (the first one does both in trained models) the answer is what the rest add up to; halves
-// have 11 bits from 2^-14 on only. 128 sequences of up to 8000 positions, bf16 rows: 158 us, in halves 139, in two pieces 174. (Halves in bands of 2^24, those
-// below the first weighed by themselves: 150, and up to 190 where scores lie far apart.)
+// A probability may have any magnitude: where one position outweighs the rest and brings next to nothing (the first one does both in trained models) the answer
+// is what the rest add up to. bf16 has that range. Halves, which the codes of V come to at less cost, have 11 bits from 2^-14 to 2^15: so over 4-bit
+// pages the codes of V are widened to bf16 too, but for up to four bf16 rows, whose probabilities are halves in two bands (page_values).
 constexpr int kSplitWarps = 8;
 constexpr float kLazy = 8.f;         // log2 of how far a score may pass the running maximum before it is moved
 
@@ -275,19 +274,55 @@ __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const ui
     for (int e = 0; e < 4; ++e) s[e] += t[e];
 }
 
-// acc[mt]: dims vdim(mt, g) of rows 2j, 2j + 1 in [0], [1], the next dim in [2], [3] (4-bit pages: a 256th of them, as widen_codes has it)
-template <typename KVT, int HD, int PP>
+// Up to four bf16 rows over 4-bit pages leave half of an MMA's columns empty. Those hold the rows again (PAIR, lanes with j >= 2), their weights times 2^24
+// and only those below 2^-13, while the first four hold the others: 52 bits of range as halves for one MMA. Relative to the largest weight, which
+// stands at 2^13 to 2^15, all down to 2^-51 have 11 bits, and those below 2^-62 are lost. 128 sequences of up to 8000 positions, 4 rows each: 142 us;
+// with V in bf16 and two pieces 174, one piece 159 (8 bits); 139 with halves alone, which lost what lay below 2^-25. Of 8 rows each, which have bf16: 177.
+constexpr float kPairTop = 13.f, kPairLazy = 2.f, kPairUp = 16777216.f;      // log2 of a weight at the reference, and how far beyond it; 2^24
+
+// acc[mt]: dims vdim(mt, g) of rows 2j, 2j + 1 in [0], [1], the next dim in [2], [3] (4-bit pages in bf16: a 256th of them, as widen_codes has it)
+template <typename KVT, int HD, int PIECES, bool PAIR>
 __device__ __forceinline__ void page_values(const PageFrag<KVT, HD>& f, const float (&w)[4], float (&acc)[HD / 16][4]) {
     using F = PageFrag<KVT, HD>;
+    constexpr int PP = PAIR ? 1 : PIECES;
     uint32_t p0[PP], p1[PP];
-    pieces(w[0], w[1], p0);
-    pieces(w[2], w[3], p1);
+    if constexpr (PAIR) {
+        // (a weight next to 2^-13 is the same number in both lanes and rounds to the same 11 bits in both bands, and so falls to one)
+        const bool second = threadIdx.x & 2;
+        const uint32_t flip = second ? 0xffffffffu : 0u, at = second ? 0x68006800u : 0x08000800u;      // 2^11, 2^-13
+        const float up = second ? kPairUp : 1.f;
+        auto band = [&](float x, float y) {
+            const uint32_t h = f32x2_to_f16(x * up, y * up);
+            return h & (__hge2_mask(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&at)) ^ flip);
+        };
+        p0[0] = band(w[0], w[1]);
+        p1[0] = band(w[2], w[3]);
+    } else {
+        pieces(w[0], w[1], p0);
+        pieces(w[2], w[3], p1);
+    }
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
         p0[i] = movmatrix(p0[i]);
         p1[i] = movmatrix(p1[i]);
     }
-    if constexpr (F::Q4) {
+    if constexpr (PAIR) {
+        const uint32_t s0 = e4m3x2_to_f16(f.vs[0]), s1 = e4m3x2_to_f16(f.vs[1]);
+#pragma unroll
+        for (int w8 = 0; w8 < F::VW; ++w8) {
+            // codes of one dim and two neighbouring rows side by side, of even dims, of odd ones
+            uint32_t h[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const uint32_t x = f.v[i][w8], y = f.v[i + 1][w8];
+                e2m1x8_to_f16((x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u), h[i]);
+                e2m1x8_to_f16((x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), h[i + 1]);
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                mma_f16(acc[w8 * 4 + m], hmul2(h[0][m], s0), hmul2(h[1][m], s0), hmul2(h[2][m], s1), hmul2(h[3][m], s1), p0[0], p1[0]);
+        }
+    } else if constexpr (F::Q4) {
         const uint32_t h0 = e4m3x2_to_f16(f.vs[0]), h1 = e4m3x2_to_f16(f.vs[1]);
         const uint32_t s0 = f32x2_to_bf16(f16_lo(h0) * kScaleUp, f16_hi(h0) * kScaleUp), s1 = f32x2_to_bf16(f16_lo(h1) * kScaleUp, f16_hi(h1) * kScaleUp);
 #pragma unroll
@@ -322,10 +357,11 @@ struct Block {
 };
 
 template <typename RT, int QP, int HD, typename F>
-__device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Block& k, uint2* qf, float* qscale, int lane) {
+__device__ __forceinline__ void pack_queries(const AttnPagedParams& p, const Block& k, bool pair, uint2* qf, float* qscale, int lane) {
     const int g = lane >> 2, j = lane & 3;                   // the B operand's column is a row of the block
-    const bool in = g < k.count;
-    const int r = k.first + (in ? g : 0), row = k.s.r0 + r / p.group, h = k.kvh * p.group + r % p.group;
+    const int i = pair ? g & 3 : g;
+    const bool in = i < k.count;
+    const int r = k.first + (in ? i : 0), row = k.s.r0 + r / p.group, h = k.kvh * p.group + r % p.group;
     const RT* q = static_cast<const RT*>(p.q) + (size_t)row * p.q_stride + (size_t)h * HD;
     // four neighbouring dims for each k-step, all on their way at once
     float x[HD / 16][4];
@@ -377,7 +413,9 @@ template <typename KVT, typename RT, int HD>
 struct SplitShape {
     using F = PageFrag<KVT, HD>;
     static constexpr int QP = sizeof(RT) == 2 ? 1 : F::Q4 ? 2 : 3;
-    static constexpr int PP = sizeof(RT) == 4 ? 3 : F::Q4 ? 1 : 2;
+    static constexpr int PP = sizeof(RT) == 4 ? 3 : 2;
+    static constexpr bool MAY_PAIR = F::Q4 && PP == 2;
+    __device__ static bool pair(int count) { return MAY_PAIR && count <= 4; }
     static constexpr int QWORDS = QP * (HD / 16) * 32;       // uint2 of a warp's queries
     static constexpr int W = HD + 2;                         // floats of a row's partial result: its sums, maximum, total
     static constexpr int PART = 8 * W;
@@ -467,9 +505,9 @@ struct PageSource<fp4_t, HD> {
     }
 };
 // The pages v, v + step, .. < v1 of a span for a block; results in acc, m (log2 of the reference of the weights) and l
-template <typename KVT, typename RT, int HD>
-__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, PageSource<KVT, HD>& src,
-                                           const uint2* qf, const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
+template <typename KVT, typename RT, int HD, bool PAIR>
+__device__ __forceinline__ void walk_rows(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, PageSource<KVT, HD>& src,
+                                          const uint2* qf, const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
     using S = SplitShape<KVT, RT, HD>;
     const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
 #pragma unroll
@@ -484,8 +522,9 @@ __device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block
     }
     const int pos0 = k.s.len - k.s.n;
     int pos[2];
-    pos[0] = 2 * j < k.count ? pos0 + (k.first + 2 * j) / p.group : -1;
-    pos[1] = 2 * j + 1 < k.count ? pos0 + (k.first + 2 * j + 1) / p.group : -1;
+    const int i0 = PAIR ? 2 * j & 3 : 2 * j;                 // this lane's first row
+    pos[0] = i0 < k.count ? pos0 + (k.first + i0) / p.group : -1;
+    pos[1] = i0 + 1 < k.count ? pos0 + (k.first + i0 + 1) / p.group : -1;
     const int low = pos0 + k.first / p.group, high = pos0 + (k.first + k.count - 1) / p.group;      // positions of the block's rows
     const float c0 = qscale[2 * j], c1 = qscale[2 * j + 1];
     PageFrag<KVT, HD>& f = src.f;
@@ -510,7 +549,8 @@ __device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block
             }
         }
         const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
-        if (__any_sync(0xffffffffu, t0 > m[0] + kLazy || t1 > m[1] + kLazy)) {
+        constexpr float lazy = PAIR ? kPairLazy : kLazy, top = PAIR ? kPairTop : 0.f;
+        if (__any_sync(0xffffffffu, t0 > m[0] + lazy || t1 > m[1] + lazy)) {
             float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
@@ -523,18 +563,37 @@ __device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block
 #pragma unroll
             for (int t = 0; t < HD / 16; ++t) { acc[t][0] *= f0; acc[t][1] *= f1; acc[t][2] *= f0; acc[t][3] *= f1; }
         }
-        const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];      // (nothing seen yet)
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0] - top, r1 = m[1] == -INFINITY ? 0.f : m[1] - top;      // (nothing seen yet)
         s[0] = ex2(s[0] - r0); s[1] = ex2(s[1] - r1); s[2] = ex2(s[2] - r0); s[3] = ex2(s[3] - r1);
         l[0] += s[0] + s[2];
         l[1] += s[1] + s[3];
-        page_values<KVT, HD, S::PP>(f, s, acc);
+        page_values<KVT, HD, S::PP, PAIR>(f, s, acc);
     }
     src.end();
+    if constexpr (PAIR) {                                    // both bands together
+        const float f = (j & 2 ? 1.f / kPairUp : 1.f) / kCodeScale;
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[t][e] *= f;
+                acc[t][e] += __shfl_xor_sync(0xffffffffu, acc[t][e], 2);
+            }
+    }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
         l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
         l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
     }
+}
+
+template <typename KVT, typename RT, int HD>
+__device__ __forceinline__ void walk_pages(const AttnPagedParams& p, const Block& k, const PagedSpan& span, int v, int v1, int step, PageSource<KVT, HD>& src,
+                                           const uint2* qf, const float* qscale, float (&acc)[HD / 16][4], float (&m)[2], float (&l)[2]) {
+    using S = SplitShape<KVT, RT, HD>;
+    if constexpr (S::MAY_PAIR)
+        if (S::pair(k.count)) return walk_rows<KVT, RT, HD, true>(p, k, span, v, v1, step, src, qf, qscale, acc, m, l);
+    walk_rows<KVT, RT, HD, false>(p, k, span, v, v1, step, src, qf, qscale, acc, m, l);
 }
 
 // Shared memory of a CTA's rings, and of its warps' results, which lie over them
@@ -577,7 +636,7 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
 // head, block of rows) are laid end to end and cut into as many equal shares as there are teams (a CTA's warps together, or each warp alone),
 // and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Bound by HBM with many bf16 pages: 64 sequences in
 // a window of 4096, 32 / 8 heads of 128, 164 us for 932 MB, 87 % of the measured copy rate. By the instructions that widen the codes with 4-bit
-// pages: 128 sequences of up to 8000 positions, the same heads, 159 us for 602 MB, 58 %. By latency (lengths, queries, page ids, pages, the
+// pages: 128 sequences of up to 8000 positions, the same heads, 142 us for 602 MB, 65 %. By latency (lengths, queries, page ids, pages, the
 // CTA's results, the join: some 1 to 2 us each) with few: one user in a window of 1024, 9 us. Sequences of more than
 // kSplitRows (token, head) pairs are left to the kernels for prompts.
 // (sequences, pages of their items before them) -> plan in shared memory; returns the total
@@ -717,7 +776,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_split_kernel(const _
         const int mine0 = v0 + (TEAM > 1 ? warp : 0);
         PageSource<KVT, HD> page(p, k, span, mine0, min(v1, span.count), TEAM, ring + warp * PageSource<KVT, HD>::kRing);
         __syncwarp();
-        pack_queries<RT, S::QP, HD, typename S::F>(p, k, const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
+        pack_queries<RT, S::QP, HD, typename S::F>(p, k, S::pair(k.count), const_cast<uint2*>(qf), const_cast<float*>(qscale), lane);
         __syncwarp();
         float acc[HD / 16][4], m[2], l[2];
         walk_pages<KVT, RT, HD>(p, k, span, mine0, min(v1, span.count), TEAM, page, qf, qscale, acc, m, l);
@@ -973,7 +1032,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     const int pos0 = k.s.len - k.s.n;
     const PagedSpan span = paged_span(p, pos0 + k.first / p.group, pos0 + (k.first + k.count - 1) / p.group);
     PageSource<KVT, HD> page(p, k, span, warp, span.count, kSplitWarps, ring + warp * PageSource<KVT, HD>::kRing);
-    if (warp == 0) pack_queries<RT, S::QP, HD, typename S::F>(p, k, qf, qscale, lane);
+    if (warp == 0) pack_queries<RT, S::QP, HD, typename S::F>(p, k, S::pair(k.count), qf, qscale, lane);
     __syncthreads();
     float acc[HD / 16][4], m[2], l[2];
     walk_pages<KVT, RT, HD>(p, k, span, warp, span.count, kSplitWarps, page, qf, qscale, acc, m, l);

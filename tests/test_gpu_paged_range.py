@@ -320,3 +320,32 @@ def test_fp32_rows_to_fp32(api, ops, cache, hd, new, batch, length):
         assert float(((got - o).abs() / t).max()) <= 1
         r0 += n
     ops.status()
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("heads", [1, 4, 7])
+def test_weights_next_to_a_band(api, ops, rows, heads):
+    """4 bits, one key far above the rest and all others alike, at every hundredth of a power of two around the border of the bands that halves are taken
+    in (2^-26 of the largest): what the others add up to is there at each."""
+    import torch
+    L, above = 500, torch.arange(24.0, 30.0, 0.01, device="cuda")
+    c = Case(api, [1] * len(above), [L] * len(above), heads, 1, 64, "fp4", rows, k_scale=1.0, v_scale=1.0, ragged=False)
+    c.table[:] = c.table[0]
+    first = int(c.table[0, 0])
+    c.kpool.zero_()
+    c.kscale.copy_(torch.ones(c.kscale.shape, device="cuda"))
+    c.kpool[first, :, 0, 0] = 0x02
+    c.vpool[first, :, 0] = 0
+    c.q.zero_()
+    c.q.view(len(above), heads, 64)[:, :, 0] = (above * math.log(2) * 8)[:, None].to(c.dt)
+    out = attend(ops, c).double().reshape(len(above), heads, 64)
+    x = c.q.view(len(above), heads, 64)[:, :, 0].double() / 8
+    v = c.cached("v", 0, L)[0].sum(0)                # of 499 equal weights
+    want = torch.exp(-x)[..., None] * v / (1 + (L - 1) * torch.exp(-x))[..., None]
+    size = torch.exp(-x)[..., None] * c.cached("v", 0, L)[0].abs().sum(0)
+    # as small_weights: two factors of one product, the reference's, the exponential; sums of L / 16 steps; bf16 rows: 11 bits of a weight and the result's 8
+    t = size * U * (2 * 4 * 21 + 4 + 4 * (L / 16 + 1) + 20 + 6)
+    if rows == "bf16":
+        t = t + 1.1 * U16 * (want.abs() + size)
+    assert float(((out - want).abs() / t).max()) <= 1
+    ops.status()
