@@ -339,8 +339,8 @@ int mlb_op_kv_read(mlb_ops* o, const mlb_paged_kv* kv, const mlb_new_rows* rows,
                    int64_t k_stride, void* v_out, int64_t v_stride, void* stream);
 /* Causal attention of the rows (already in the cache) over the pages: the row at position p sees position j <= p where
  * window = 0, or j > p - window (its newest `window` positions, itself among them), or j < sinks (the first ones). q and out
- * [rows][heads * head_dim] of row_dtype (out is not q), heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
- * (0: 1 / sqrt(head_dim)); gate (nullable) fp32 [rows][heads * head_dim] multiplies the output. Sums and softmax statistics are
+ * [rows][heads * head_dim] of row_dtype (out does not overlap q), heads a multiple of kv_heads, up to 8 times it; scores are multiplied by `scale`
+ * (0: 1 / sqrt(head_dim)); gate (nullable) fp32 [rows][heads * head_dim] multiplies the output (of padding rows it is not read). Sums and softmax statistics are
  * fp32; with float32 rows so is everything else to fp32's own rounding (over 4-bit pages q is taken to 22 bits, and to no finer than 2^-33 of
  * its row's largest), with bfloat16 rows probabilities may be rounded to bf16: each of them, down to 2^-50 of the row's largest. What
  * lies at positions that a row does not see (numbers or not) does not reach its output. A row whose answer is no number, or that meets an infinity, is

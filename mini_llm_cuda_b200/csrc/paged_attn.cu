@@ -619,7 +619,7 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
     y = pos < 0 ? 0.f : y * inv;
     const size_t at = (size_t)row * p.heads * HD + (size_t)h * HD + d;
     const bool odd = !(fabsf(x) <= 3.4e38f) || !(fabsf(y) <= 3.4e38f);
-    if (p.gate) { x *= p.gate[at]; y *= p.gate[at + 1]; }
+    if (p.gate && pos >= 0) { x *= p.gate[at]; y *= p.gate[at + 1]; }      // (of a padding row it may hold anything)
     RT* o = static_cast<RT*>(p.out) + (size_t)row * p.out_stride + (size_t)h * HD + d;
     if (reinterpret_cast<uintptr_t>(o) % (2 * sizeof(RT)) == 0) {
         if constexpr (sizeof(RT) == 2) *reinterpret_cast<uint32_t*>(o) = f32x2_to_bf16(x, y);

@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
                         y[u] = pos < 0 ? 0.f : __uint_as_float(o[from]) * inv;
                         odd |= !(fabsf(y[u]) <= 3.4e38f);
                     }
-                    if (p.gate && in) {
+                    if (p.gate && in && pos >= 0) {
                         const float* gp = p.gate + (size_t)row * p.heads * HD + (size_t)h * HD + e * 32;
 #pragma unroll
                         for (int u = 0; u < 32; ++u) y[u] *= gp[u];

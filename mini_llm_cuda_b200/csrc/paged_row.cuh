@@ -137,7 +137,7 @@ static __device__ __noinline__ void careful_row(const AttnPagedParams& p, int b,
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         float y = any ? o[e] / sum * p.c.v_scale : 0.f;
-        if (p.gate) y *= p.gate[(size_t)row * p.heads * HD + (size_t)h * HD + lane * E + e];
+        if (p.gate && any) y *= p.gate[(size_t)row * p.heads * HD + (size_t)h * HD + lane * E + e];
         Elem<RT>::put(op, e, y);
     }
 }

@@ -349,3 +349,52 @@ def test_weights_next_to_a_band(api, ops, rows, heads):
         t = t + 1.1 * U16 * (want.abs() + size)
     assert float(((out - want).abs() / t).max()) <= 1
     ops.status()
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 70])
+def test_padding_rows_are_zeros_whatever_their_gates(api, ops, cache, rows, new):
+    """A row before position 0 attends to nothing and is 0, though its gate and query were never written."""
+    import torch
+    lens = [max(0, new - 2), new + 20, 0]
+    c = Case(api, [new] * 3, lens, 4, 2, 64, cache, rows)
+    gate = torch.rand(c.rows, 4 * 64, device="cuda")
+    want, tol = c.attention(30, 2, gate=gate)
+    row = torch.arange(new, device="cuda")
+    padding = torch.cat([row < new - n for n in lens])
+    gate[padding] = torch.tensor([math.nan, math.inf, -math.inf, math.nan], device="cuda").repeat(64)
+    c.q[padding] = math.nan
+    out = attend(ops, c, 30, 2, gate=gate).double()
+    assert bool((out[padding] == 0).all())
+    assert float(((out - want).abs() - tol)[~padding].max()) <= 0
+    ops.status()
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_negative_scale(api, ops, cache, rows, new):
+    c = Case(api, [new, new], [new + 200, new], 8, 2, 64, cache, rows)
+    for scale in (-0.2, 1e-3):
+        want, tol = c.attention(100, 3, scale=scale)
+        # (the bound counts the scores' size by their sign)
+        size = c.attention(100, 3, scale=abs(scale))[1]
+        out = attend(ops, c, 100, 3, scale=scale).double()
+        assert float(((out - want).abs() - tol.abs().maximum(size)).max()) <= 0
+    ops.status()
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+def test_4096_sequences(api, ops, cache, rows):
+    """The most a call takes, many of them empty."""
+    rng = np.random.default_rng(3)
+    lens = (rng.integers(0, 40, size=4096) * (rng.random(4096) < 0.6)).tolist()
+    c = Case(api, [1] * 4096, lens, 2, 1, 64, cache, rows, ragged=False)
+    out = attend(ops, c, 20, 2).double()
+    ops.status()
+    pick = rng.choice(4096, size=300, replace=False).tolist() + [0, 4095]
+    for b in pick:
+        d = Case.__new__(Case)
+        d.__dict__.update(c.__dict__)
+        d.new, d.lens, d.rows, d.table, d.q = [1], [lens[b]], 1, c.table[b:b + 1], c.q[b:b + 1]
+        want, tol = d.attention(20, 2)
+        assert float(((out[b:b + 1] - want).abs() - tol).max()) <= 0
