@@ -514,7 +514,7 @@ class Ops:
         if x.get_device() != self.device:
             raise ValueError(f"{what} is not on CUDA device {self.device}")
         s = x.shape
-        if len(s) != 3 or s[0] != rows or s[1] * s[2] != width or x.stride(2) != 1 or x.stride(1) != s[2]:
+        if len(s) != 3 or s[0] != rows or s[1] * s[2] != width or x.stride(2) != 1 or s[1] != 1 and x.stride(1) != s[2]:
             raise ValueError(f"{what} must be [{rows}][{width}], dense within a row")
         return x.data_ptr(), x.stride(0)
 

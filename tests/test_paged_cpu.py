@@ -216,3 +216,20 @@ def test_numbers_beyond_32_bits(api, fake_ops):
     lens.is_cuda, lens.is_contiguous, lens.numel = True, lambda: True, lambda: 3
     assert api.NewRows(lens, 3, max_rows=(1 << 32) + 1).struct.max_rows == top
     assert api.NewRows(lens, 3, max_rows=7).struct.max_rows == 7
+
+
+def test_rows_of_one_head(api, fake_ops):
+    """[rows][1][head_dim] has no second head, so the stride to it says nothing; of more heads it has to be dense."""
+    import torch
+    ops, calls, cache, rows = fake_ops
+
+    def rows_of(shape, strides):
+        x = FakeTensor(torch.float32, 5, 128)
+        x.shape, x._stride = torch.Size(shape), strides
+        return ops._rows(x, "k", (5, 128), torch.float32)
+
+    assert rows_of((5, 1, 128), (128, 640, 1)) == (1 << 20, 128)
+    assert rows_of((5, 2, 64), (200, 64, 1)) == (1 << 20, 200)
+    for shape, strides in (((5, 2, 64), (64, 320, 1)), ((5, 1, 128), (128, 640, 2)), ((5, 1, 64), (64, 320, 1)), ((4, 1, 128), (128, 640, 1))):
+        with pytest.raises(ValueError):
+            rows_of(shape, strides)
