@@ -992,9 +992,9 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attn_blocks_kernel(const 
     __shared__ float qscale[8];
     __shared__ int found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
-    // which sequence's block this is: blocks of those with more than kSplitRows rows, one after another
+    // which sequence's block this is: blocks of those with more than kSplitRows rows, the last sequence and its later rows (which see more) first
     if (warp == 0) {
-        int want = (int)(gridDim.x - 1 - blockIdx.x), at = -1;      // later rows, which see more, first
+        int want = (int)(gridDim.x - 1 - blockIdx.x), at = -1;
         for (int b0 = 0; b0 < p.r.batch && at < 0; b0 += 32) {
             const int b = b0 + lane;
             int n = 0;
@@ -1083,8 +1083,8 @@ cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int ctas = 2 * sm_count;
     p.max_teams = TEAM == 1 ? ctas * kSplitWarps : ctas;
-    // Beside its pages an item costs what comes before and after them, measured in pages: 7 small ones of 4 bits for a warp alone (2: 153 us for 128
-    // sequences of up to 8000 positions, 4: 146, 6: 140, 8: 138; 256 short ones 63, 52, 47, 46), 4 others (2: 86 us for 200 sequences of up to 2000, 4:
+    // Beside its pages an item costs what comes before and after them, measured in pages: 7 small ones of 4 bits for a warp alone (2: 170 us for 128
+    // sequences of up to 8000 positions with weights in bf16, 4: 165, 6: 160, 8: 161; 256 short ones 68, 57, 52, 52), 4 others (2: 86 us for 200 sequences of up to 2000, 4:
     // 81, 8: 84), and two for each warp of a team (1: 172 us for 64 sequences in a window of 4096, 2: 164, 4: 166). Where a share has parts of two items at
     // most, that is the same for all and left out.
     p.item_cost = (long long)p.r.batch * p.c.kv_heads * 4 < p.max_teams ? 0 : TEAM > 1 ? 2 * TEAM : sizeof(KVT) == 1 ? 7 : 4;
@@ -1098,7 +1098,11 @@ cudaError_t split_launch(AttnPagedParams p, int sm_count, cudaStream_t st) {
 template <typename KVT, typename RT, int HD>
 cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) {
     using S = SplitShape<KVT, RT, HD>;
-    // Each warp alone where there are sequences and heads enough to give most of them whole items: nothing to put together in a CTA.
+    // Each warp alone where there are sequences and heads enough to give most of them whole items: nothing to put together in a CTA. A warp / a CTA a share,
+    // in us, 8 K/V heads, sequences of up to 3000 positions: bf16 pages, heads of 128, 464 items 78 / 77, 600 93 / 105, 1024 147 / 160, 2048 280 / 305;
+    // heads of 64 38 / 42, 46 / 55, 73 / 86, 134 / 162; fp32 pages, heads of 128, 224 / 225, 264 / 298, 437 / 489, 862 / 979; 4-bit pages, fp32 rows, heads
+    // of 128, 51 / 60, 58 / 81, 89 / 123, 168 / 233. Of up to 300 positions the warp is ahead by more (bf16, 128, 600 items: 27 / 38). So over
+    // 4-bit pages it would be from about 300 items on; one rule for all stays behind there.
     const long long items = (long long)p.r.batch * p.c.kv_heads;
     const bool prompts = paged_prompts(p.r.row_start, p.r.rows, p.r.max_rows, p.group);
     constexpr bool TILES = sizeof(KVT) <= 2 && sizeof(RT) == 2;
@@ -1108,13 +1112,16 @@ cudaError_t launch_one(const AttnPagedParams& p, int sm_count, cudaStream_t st) 
     if (e != cudaSuccess) return e;
     e = items >= 4LL * sm_count ? split_launch<KVT, RT, HD, 1>(p, sm_count, st) : split_launch<KVT, RT, HD, kSplitWarps>(p, sm_count, st);
     if (e != cudaSuccess || !prompts) return e;
-    if constexpr (TILES) return attn_prompt_launch(p, dtype, HD, maps, st);
-    const size_t smem = (size_t)S::QWORDS * 8 + split_ring_bytes<KVT, HD, kSplitWarps>();
-    e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-    if (e != cudaSuccess) return e;
-    const long long blocks = (long long)p.r.rows * p.group / 8 + p.r.batch;
-    attn_blocks_kernel<KVT, RT, HD><<<dim3((unsigned)blocks, p.c.kv_heads), 32 * kSplitWarps, smem, st>>>(p);
-    return cudaGetLastError();
+    if constexpr (TILES) {
+        return attn_prompt_launch(p, dtype, HD, maps, st);
+    } else {
+        const size_t smem = (size_t)S::QWORDS * 8 + split_ring_bytes<KVT, HD, kSplitWarps>();
+        e = cudaFuncSetAttribute(attn_blocks_kernel<KVT, RT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        if (e != cudaSuccess) return e;
+        const long long blocks = (long long)p.r.rows * p.group / 8 + p.r.batch;
+        attn_blocks_kernel<KVT, RT, HD><<<dim3((unsigned)blocks, p.c.kv_heads), 32 * kSplitWarps, smem, st>>>(p);
+        return cudaGetLastError();
+    }
 }
 
 template <typename KVT, typename RT>

@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(kPpThreads<KVT>, 3 - kPpTiles<KVT>)
         tc_fence_before();
     }
     if (warp == kLoader) {
-        // which sequence's rows these are: those of sequences with more than kSplitRows, 128 TILES at a time, later rows (which see more) first
+        // which sequence's rows these are: those of sequences with more than kSplitRows, 128 TILES at a time, the last sequence and its later rows
+        // (which see more) first; sequences are not ordered by length
         int want = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)p.c.kv_heads), at = -1;
         for (int b0 = 0; b0 < p.r.batch && at < 0; b0 += 32) {
             const int b = b0 + lane;
