@@ -21,7 +21,9 @@ namespace {
 // and its rescaling need no exchange between lanes but the maximum itself, and that only when a score passes the old one by 2^8; P is
 // turned round by movmatrix.
 // fp32 numbers are taken in pieces whose products are exact: fp32 queries, K, V and probabilities in three bf16, probabilities of bf16 rows in two. Products of
-// pieces below 2^-24 of the whole are left out. 4-bit codes times their e4m3 scale are exact halves, to which the conversion instruction brings them, and meet
+// pieces below 2^-24 of the whole are left out. Matrix cores cut off where they add, at the size of what they add to: the products of pieces behind the first have
+// sums of their own in a score, and with fp32 rows a page's values are summed by themselves and added to the pages' before it in fp32 (error against 64 bits 2e-7 to
+// 5e-7 of the answer, 5e-7 to 2e-6 with everything in one sum, at 0 to 8 % of the time). 4-bit codes times their e4m3 scale are exact halves, to which the conversion instruction brings them, and meet
 // queries as halves (fp32: two of them, bf16: one), the row scaled by a power of two to lie within their range.
 // A probability may have any magnitude: where one position outweighs the rest and brings next to nothing (the first one does both in trained models) the answer
 // is what the rest add up to. bf16 has that range. Halves, which the codes of V come to at less cost, have 11 bits from 2^-14 to 2^15: so over 4-bit
@@ -244,7 +246,7 @@ struct PageFrag<fp4_t, HD> {
 template <typename KVT, int HD, int QP>
 __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const uint2* qf, int lane, float (&s)[4]) {
     using F = PageFrag<KVT, HD>;
-    float t[4] = {0.f, 0.f, 0.f, 0.f};                       // two chains of products
+    float t[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};       // two chains of products, and those of pieces behind the first
     s[0] = s[1] = s[2] = s[3] = 0.f;
     if constexpr (F::Q4) {
         uint32_t h[2][HD / 8];
@@ -254,7 +256,7 @@ __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const ui
 #pragma unroll
             for (int i = 0; i < QP; ++i) {
                 const uint2 b = qf[(i * (HD / 16) + ks) * 32 + lane];
-                mma_f16(ks % 2 ? t : s, h[0][2 * ks], h[1][2 * ks], h[0][2 * ks + 1], h[1][2 * ks + 1], b.x, b.y);
+                mma_f16(i > 0 ? low : ks % 2 ? t : s, h[0][2 * ks], h[1][2 * ks], h[0][2 * ks + 1], h[1][2 * ks + 1], b.x, b.y);
             }
     } else {
 #pragma unroll
@@ -266,12 +268,12 @@ __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const ui
                 const uint2 b = qf[(i * (HD / 16) + ks) * 32 + lane];
 #pragma unroll
                 for (int k = 0; k < F::KP; ++k)
-                    if (i + k < 3) mma_bf16((ks + i) % 2 ? t : s, a[k][0], a[k][1], a[k][2], a[k][3], b.x, b.y);
+                    if (i + k < 3) mma_bf16(i + k > 0 ? low : ks % 2 ? t : s, a[k][0], a[k][1], a[k][2], a[k][3], b.x, b.y);
             }
         }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] += t[e];
+    for (int e = 0; e < 4; ++e) s[e] = QP > 1 || F::KP > 1 ? s[e] + t[e] + low[e] : s[e] + t[e];
 }
 
 // Up to four bf16 rows over 4-bit pages leave half of an MMA's columns empty. Those hold the rows again (PAIR, lanes with j >= 2), their weights times 2^24
@@ -330,22 +332,30 @@ __device__ __forceinline__ void page_values(const PageFrag<KVT, HD>& f, const fl
             // four dims of two neighbouring rows, the one's codes under the other's: widen_codes puts a dim's two together
             const int sel = w % 2 ? 0x7632 : 0x5410;
             const uint4 x = widen_codes(__byte_perm(f.v[0][w / 2], f.v[1][w / 2], sel), s0), y = widen_codes(__byte_perm(f.v[2][w / 2], f.v[3][w / 2], sel), s1);
+            float own[2][4] = {};                            // the page's, smallest products first
 #pragma unroll
-            for (int i = 0; i < PP; ++i) {
-                mma_bf16(acc[w * 2], x.x, x.y, y.x, y.y, p0[i], p1[i]);
-                mma_bf16(acc[w * 2 + 1], x.z, x.w, y.z, y.w, p0[i], p1[i]);
+            for (int i = PP - 1; i >= 0; --i) {
+                mma_bf16(PP == 3 ? own[0] : acc[w * 2], x.x, x.y, y.x, y.y, p0[i], p1[i]);
+                mma_bf16(PP == 3 ? own[1] : acc[w * 2 + 1], x.z, x.w, y.z, y.w, p0[i], p1[i]);
             }
+            if constexpr (PP == 3)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { acc[w * 2][e] += own[0][e]; acc[w * 2 + 1][e] += own[1][e]; }
         }
     } else {
 #pragma unroll
         for (int mt = 0; mt < HD / 16; ++mt) {
             uint32_t a[F::KP][4];
+            float own[4] = {};
             f.v_operand(mt, a);
 #pragma unroll
-            for (int k = 0; k < F::KP; ++k)
+            for (int o = 2; o >= 0; --o)                     // pieces o - k of the weights and k of V
 #pragma unroll
-                for (int i = 0; i < PP; ++i)
-                    if (i + k < 3) mma_bf16(acc[mt], a[k][0], a[k][1], a[k][2], a[k][3], p0[i], p1[i]);
+                for (int k = 0; k < F::KP; ++k)
+                    if (k <= o && o - k < PP) mma_bf16(PP == 3 ? own : acc[mt], a[k][0], a[k][1], a[k][2], a[k][3], p0[o - k], p1[o - k]);
+            if constexpr (PP == 3)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[mt][e] += own[e];
         }
     }
 }

@@ -398,3 +398,32 @@ def test_4096_sequences(api, ops, cache, rows):
         d.new, d.lens, d.rows, d.table, d.q = [1], [lens[b]], 1, c.table[b:b + 1], c.q[b:b + 1]
         want, tol = d.attention(20, 2)
         assert float(((out[b:b + 1] - want).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("cache", ["f32", "bf16", "fp4"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,batch,length", [(1, 1, 6000), (1, 300, 900), (40, 2, 1500)])
+def test_fp32_error_as_a_whole(api, ops, cache, hd, new, batch, length):
+    """fp32 rows: the error of all numbers together, against that of the same formula in plain fp32 torch operations. Both round at random, within half a step of what
+    they add to; cutting off instead, a whole step always to the same side, gives several times as much. Twice the plain form's is allowed."""
+    import torch
+    c = Case(api, [new] * batch, [length] * batch, 4, 2, hd, cache, "f32", seed=4)
+    if cache == "fp4":
+        c.k_scale, c.v_scale = 0.02, 0.02
+        c.describe()
+    out = attend(ops, c)
+    KH, G, r0, mine, plain = c.kv_heads, c.heads // c.kv_heads, 0, 0.0, 0.0
+    for b, (n, L) in enumerate(zip(c.new, c.lens)):
+        q = c.q[r0:r0 + n].double().reshape(n, KH, G, hd).permute(1, 2, 0, 3)
+        K, V = c.cached("k", b, L)[:, None], c.cached("v", b, L)[:, None]
+        hidden = torch.arange(L, device="cuda")[None] > torch.arange(L - n, L, device="cuda")[:, None]
+        forms = []
+        for t in (torch.float64, torch.float32):
+            s = (q.to(t) @ K.to(t).transpose(-1, -2) * (1 / math.sqrt(hd))).masked_fill(hidden, -math.inf)
+            forms.append((torch.softmax(s, dim=-1) @ V.to(t)).double())
+        got = out[r0:r0 + n].double().reshape(n, KH, G, hd).permute(1, 2, 0, 3)
+        mine += float(((got - forms[0]) ** 2).sum())
+        plain += float(((forms[1] - forms[0]) ** 2).sum())
+        r0 += n
+    assert mine <= 4 * plain, (math.sqrt(mine / plain))
+    ops.status()
