@@ -645,9 +645,9 @@ __device__ __forceinline__ bool put_pair(const AttnPagedParams& p, int row, int 
 // Page counts of a batch's sequences differ, and so does how many sequences there are for 148 SMs: so the pages of all (sequence, K/V
 // head, block of rows) are laid end to end and cut into as many equal shares as there are teams (a CTA's warps together, or each warp alone),
 // and the shares' partial results of an item that a cut goes through are put together by attn_join_kernel. Bound by HBM with many bf16 pages: 64 sequences in
-// a window of 4096, 32 / 8 heads of 128, 164 us for 932 MB, 87 % of the measured copy rate. By the instructions that widen the codes with 4-bit
-// pages: 128 sequences of up to 8000 positions, the same heads, 142 us for 602 MB, 65 %. By latency (lengths, queries, page ids, pages, the
-// CTA's results, the join: some 1 to 2 us each) with few: one user in a window of 1024, 9 us. Sequences of more than
+// a window of 4096, 32 / 8 heads of 128, 167 us for 932 MB, 85 % of the measured copy rate. By the instructions that widen the codes with 4-bit
+// pages: 128 sequences of up to 8000 positions, the same heads, 144 us for 602 MB, 64 %. By latency (lengths, queries, page ids, pages, the
+// CTA's results, the join: some 1 to 2 us each) with few: one user in a window of 1024, 10 us. Sequences of more than
 // kSplitRows (token, head) pairs are left to the kernels for prompts.
 // (sequences, pages of their items before them) -> plan in shared memory; returns the total
 __device__ __forceinline__ int split_blocks(const AttnPagedParams& p, int n) {

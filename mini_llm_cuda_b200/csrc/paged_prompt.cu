@@ -13,7 +13,7 @@
 //
 // What bounds it (bf16, heads of 128): not the tensor core (36 % of its cycles in the window below), the exponential's unit (32 %) or the issue slots (46 %), but the chain
 // softmax -> P V -> next scores of each tile, 3500 cycles of which two tiles overlap; tensor memory holds no third tile and no second S. 8001
-// tokens, 16 / 4 heads of 128: 262 us, 1000 TFLOP/s; in a window of 1024 104 us, 590 TFLOP/s, where a CTA's start and end (6 us of 26) tell.
+// tokens, 16 / 4 heads of 128: 262 us, 1000 TFLOP/s; in a window of 1024 104 us, 613 TFLOP/s, where a CTA's start and end (6 us of 26) tell.
 #include <cstring>
 #include <type_traits>
 
