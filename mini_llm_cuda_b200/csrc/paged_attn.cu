@@ -276,11 +276,11 @@ __device__ __forceinline__ void page_scores(const PageFrag<KVT, HD>& f, const ui
     for (int e = 0; e < 4; ++e) s[e] = QP > 1 || F::KP > 1 ? s[e] + t[e] + low[e] : s[e] + t[e];
 }
 
-// Up to four bf16 rows over 4-bit pages leave half of an MMA's columns empty. Those hold the rows again (PAIR, lanes with j >= 2), their weights times 2^24
-// and only those below 2^-13, while the first four hold the others: 52 bits of range as halves for one MMA. Relative to the largest weight, which
-// stands at 2^13 to 2^15, all down to 2^-51 have 11 bits, and those below 2^-62 are lost. 128 sequences of up to 8000 positions, 4 rows each: 142 us;
+// Up to four bf16 rows over 4-bit pages leave half of an MMA's columns empty. The first four hold a row's weights times 2^13 from 2^-13 on, the others the row
+// again (PAIR, lanes with j >= 2) with those below, times 2^37: 52 bits of range as halves for one MMA. Relative to the largest weight, which
+// stands at 2^13 to 2^15 there, all down to 2^-51 have 11 bits, and those below 2^-62 are lost. 128 sequences of up to 8000 positions, 4 rows each: 144 us;
 // with V in bf16 and two pieces 174, one piece 159 (8 bits); 139 with halves alone, which lost what lay below 2^-25. Of 8 rows each, which have bf16: 177.
-constexpr float kPairTop = 13.f, kPairLazy = 2.f, kPairUp = 16777216.f;      // log2 of a weight at the reference, and how far beyond it; 2^24
+constexpr float kPairUp = 8192.f, kPairLow = 137438953472.f, kPairLazy = 2.f;      // 2^13, 2^37; log2 of how far a score may pass the running maximum
 
 // acc[mt]: dims vdim(mt, g) of rows 2j, 2j + 1 in [0], [1], the next dim in [2], [3] (4-bit pages in bf16: a 256th of them, as widen_codes has it)
 template <typename KVT, int HD, int PIECES, bool PAIR>
@@ -292,7 +292,7 @@ __device__ __forceinline__ void page_values(const PageFrag<KVT, HD>& f, const fl
         // (a weight next to 2^-13 is the same number in both lanes and rounds to the same 11 bits in both bands, and so falls to one)
         const bool second = threadIdx.x & 2;
         const uint32_t flip = second ? 0xffffffffu : 0u, at = second ? 0x68006800u : 0x08000800u;      // 2^11, 2^-13
-        const float up = second ? kPairUp : 1.f;
+        const float up = second ? kPairLow : kPairUp;
         auto band = [&](float x, float y) {
             const uint32_t h = f32x2_to_f16(x * up, y * up);
             return h & (__hge2_mask(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&at)) ^ flip);
@@ -559,7 +559,7 @@ __device__ __forceinline__ void walk_rows(const AttnPagedParams& p, const Block&
             }
         }
         const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
-        constexpr float lazy = PAIR ? kPairLazy : kLazy, top = PAIR ? kPairTop : 0.f;
+        constexpr float lazy = PAIR ? kPairLazy : kLazy;
         if (__any_sync(0xffffffffu, t0 > m[0] + lazy || t1 > m[1] + lazy)) {
             float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
 #pragma unroll
@@ -573,7 +573,7 @@ __device__ __forceinline__ void walk_rows(const AttnPagedParams& p, const Block&
 #pragma unroll
             for (int t = 0; t < HD / 16; ++t) { acc[t][0] *= f0; acc[t][1] *= f1; acc[t][2] *= f0; acc[t][3] *= f1; }
         }
-        const float r0 = m[0] == -INFINITY ? 0.f : m[0] - top, r1 = m[1] == -INFINITY ? 0.f : m[1] - top;      // (nothing seen yet)
+        const float r0 = m[0] == -INFINITY ? 0.f : m[0], r1 = m[1] == -INFINITY ? 0.f : m[1];      // (nothing seen yet)
         s[0] = ex2(s[0] - r0); s[1] = ex2(s[1] - r1); s[2] = ex2(s[2] - r0); s[3] = ex2(s[3] - r1);
         l[0] += s[0] + s[2];
         l[1] += s[1] + s[3];
@@ -581,7 +581,7 @@ __device__ __forceinline__ void walk_rows(const AttnPagedParams& p, const Block&
     }
     src.end();
     if constexpr (PAIR) {                                    // both bands together
-        const float f = (j & 2 ? 1.f / kPairUp : 1.f) / kCodeScale;
+        const float f = 1.f / ((j & 2 ? kPairLow : kPairUp) * kCodeScale);
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t)
 #pragma unroll

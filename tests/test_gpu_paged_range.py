@@ -427,3 +427,36 @@ def test_fp32_error_as_a_whole(api, ops, cache, hd, new, batch, length):
         r0 += n
     assert mine <= 4 * plain, (math.sqrt(mine / plain))
     ops.status()
+
+
+@pytest.mark.parametrize("cache,rows", TYPES)
+@pytest.mark.parametrize("new", [1, 6, 60])
+def test_scores_past_fp32_steps_of_one(api, ops, cache, rows, new):
+    """Scores of some 10^8, where fp32's own steps are 8 and more: the largest takes all the weight; with its sign turned it has none."""
+    import torch
+    L = 300 + new
+    c = Case(api, [new], [L], 4, 2, 64, cache, rows)
+    key = 3                                             # slot 7 of this page stands out, by dim 0
+    c.kpool.zero_()
+    if cache == "fp4":
+        c.kscale.copy_(torch.ones(c.kscale.shape, device="cuda"))
+        c.kpool[c.table[0, key].long(), :, 7, 0] = 0x02
+        c.k_scale = 1.0
+    else:
+        c.kpool[c.table[0, key].long(), :, 7, 0] = 1
+    c.describe()
+    c.q.zero_()
+    c.q.view(new, 4, 64)[:, :, 0] = 1e9
+    want = c.cached("v", 0, L)[:, key * 16 + 7].repeat_interleave(2, 0)[None].expand(new, -1, -1)
+    out = attend(ops, c).double().view(new, 4, 64)
+    t = want.abs() * (U16 * 1.1 * 2 if rows == "bf16" else U * 40)
+    assert float(((out - want).abs() - t).max()) <= 0
+    c.q.neg_()                                          # now that one is out, and all others weigh the same
+    out = attend(ops, c).double().view(new, 4, 64)
+    for i in range(new):
+        keep = torch.arange(L - new + i + 1, device="cuda") != key * 16 + 7
+        v = c.cached("v", 0, L - new + i + 1)[:, keep]
+        mean, size = (x.mean(1).repeat_interleave(2, 0) for x in (v, v.abs()))
+        t = size * U * (4 * (L / 16 + 1) + 40) + (1.1 * U16 * (size + mean.abs()) if rows == "bf16" else 0)
+        assert float(((out[i] - mean).abs() - t).max()) <= 0
+    ops.status()
